@@ -18,6 +18,7 @@ _lib: Optional[C.CDLL] = None
 _p = C.c_void_p
 _i = C.c_int
 _sz = C.c_size_t
+_f = C.c_float
 
 # name -> (restype, argtypes); mirrors include/ccfuser_moe.h declaration by declaration
 SIGNATURES = {
@@ -65,6 +66,11 @@ SIGNATURES = {
     "ccf_ffn2_forward_kn": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p, _sz, _p]),
     "ccf_ffn1_forward_opts": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _i, _i, _p, _p, _sz, _p]),
     "ccf_ffn2_forward_opts": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _i, _p, _p, _sz, _p]),
+    "ccf_rms_norm": (_i, [_p, _p, _p, _i, _i, _f, _i, _i, _p, _p, _p, _p, _p, _p]),
+    "ccf_rms_norm_backward_workspace_bytes": (_sz, [_i, _i]),
+    "ccf_rms_norm_backward": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
+    "ccf_quantize_rows": (_i, [_p, _i, _i, _i, _p, _p, _p]),
+    "ccf_quantize_weight": (_i, [_p, _i, _i, _i, _i, _p, _p, _p]),
 }
 
 

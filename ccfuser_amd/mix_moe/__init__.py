@@ -8,7 +8,8 @@ be 1 and nothing here opens a communicator.
 from .gates import BaseGate, NaiveGate
 from .layers import MixMOE
 from .linear import FMoELinear, MixMOEInstance, MixMOELinear1, MixMOELinear2
+from .norm import RMSNorm, rms_norm
 from .transformer import AsyncExpertAssignment, MixMOETransformerMLP
 
 __all__ = ["BaseGate", "NaiveGate", "MixMOE", "FMoELinear", "MixMOEInstance", "MixMOELinear1",
-           "MixMOELinear2", "AsyncExpertAssignment", "MixMOETransformerMLP"]
+           "MixMOELinear2", "AsyncExpertAssignment", "MixMOETransformerMLP", "RMSNorm", "rms_norm"]

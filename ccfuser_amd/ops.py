@@ -9,13 +9,13 @@ mix_moe/csrc/mix_moe.h:242-245, or asserts, mix_moe/csrc/cuda/utils.h:4-6).
 from __future__ import annotations
 
 import contextlib
-from typing import Dict, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
 
-CCF_F16, CCF_F32 = 0, 1
+CCF_F16, CCF_F32, CCF_BF16 = 0, 1, 2
 CCF_FFN_KN, CCF_FFN_IN_LAYER = 1, 2
 
 
@@ -716,3 +716,133 @@ def moe_ffn_blocks(x, pos, expert_ids, lens, start_addrs, block_size: int, top_k
                   _ptr(start_addrs), nb, int(block_size), d, f, E, _ptr(w1), int(w1_kn), _ptr(b1), _ptr(w2),
                   int(w2_kn), _ptr(b2), _ptr(y), _ptr(ws), ws.numel(), _stream(x))
     return y
+
+
+# --------------------------------------------------- norm and 8-bit rows
+_TYPE_CODES = {torch.float16: CCF_F16, torch.float32: CCF_F32, torch.bfloat16: CCF_BF16}
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128              # elements of a row, or rows and columns of a weight's block, that share a scale
+
+
+def _scale_blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+def _type_code(t: torch.Tensor, name: str) -> int:
+    code = _TYPE_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
+    return code
+
+
+def _same_device(first: torch.Tensor, *others) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+
+
+class NormOutput(NamedTuple):
+    """What ``rms_norm`` returns; None for what was not asked for."""
+    y: Optional[torch.Tensor]           # [..., d], the rows' type
+    total: torch.Tensor                 # x + residual, or x itself
+    codes: Optional[torch.Tensor]       # [..., d] float8_e4m3fn
+    scale: Optional[torch.Tensor]       # [..., ceil(d / 128)] float32
+    rstd: Optional[torch.Tensor]        # [rows] float32
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None,
+             want_y: bool = True, want_fp8: bool = False, want_rstd: bool = False) -> NormOutput:
+    """Root-mean-square norm over the last dimension of ``x`` (fp16, bf16 or fp32), after the addition of ``residual``, whose
+    rounded sum is returned as ``total``.  ``want_fp8`` also gives the result in e4m3 with a scale for each 128 columns, as
+    ``quantize_rows`` would make it of the unrounded result.  ``weight`` [d] has x's type or is fp32.  Not differentiable
+    (``mix_moe.rms_norm`` is)."""
+    _check(x, "x")
+    code = _type_code(x, "x")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("rms_norm: x has no columns")
+    _check(weight, "weight", ndim=1)
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"weight must be {x.dtype} or float32, got {weight.dtype}")
+    d = x.shape[-1]
+    if weight.shape[0] != d:
+        raise ValueError("rms_norm: x and weight do not match")
+    if residual is not None:
+        _check(residual, "residual", dtype=x.dtype)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    if not (want_y or want_fp8):
+        raise ValueError("rms_norm: neither y nor its 8-bit form is wanted")
+    _same_device(x, weight, residual)
+    rows, dev = x.numel() // d, x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_y else None
+    total = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+    codes = torch.empty(x.shape, dtype=FP8, device=dev) if want_fp8 else None
+    scale = torch.empty(*x.shape[:-1], _scale_blocks(d), dtype=torch.float32, device=dev) if want_fp8 else None
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if want_rstd else None
+    with _on(x):
+        _lib.call("ccf_rms_norm", _ptr(x), _ptr(residual), _ptr(weight), rows, d, float(eps), code,
+                  _TYPE_CODES[weight.dtype], _ptr(y), _ptr(total), _ptr(codes), _ptr(scale), _ptr(rstd), _stream(x))
+    return NormOutput(y, x if total is None else total, codes, scale, rstd)
+
+
+def rms_norm_backward(grad_y: torch.Tensor, total: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                      grad_total: Optional[torch.Tensor] = None, want_x: bool = True,
+                      want_weight: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(grad_x, grad_weight) of ``rms_norm``, each None when not wanted; grad_x is the gradient of x and of the residual.
+    ``grad_total``: the gradient that reaches ``total`` by other ways."""
+    _check(total, "total")
+    code = _type_code(total, "total")
+    _check(grad_y, "grad_y", dtype=total.dtype)
+    _check(weight, "weight", ndim=1)
+    _check(rstd, "rstd", dtype=torch.float32, ndim=1)
+    if weight.dtype not in (total.dtype, torch.float32):
+        raise TypeError(f"weight must be {total.dtype} or float32, got {weight.dtype}")
+    d = weight.shape[0]
+    if d == 0 or total.dim() < 1 or total.shape[-1] != d or grad_y.shape != total.shape or rstd.numel() != total.numel() // d:
+        raise ValueError("rms_norm_backward: shapes do not match")
+    if grad_total is not None:
+        _check(grad_total, "grad_total", dtype=total.dtype)
+        if grad_total.shape != total.shape:
+            raise ValueError("rms_norm_backward: shapes do not match")
+    _same_device(total, grad_y, weight, rstd, grad_total)
+    if not (want_x or want_weight):
+        return None, None
+    rows = total.numel() // d
+    g_x = torch.empty_like(total) if want_x else None
+    g_w = torch.empty_like(weight) if want_weight else None
+    with _on(total):
+        ws = _workspace(_lib.lib().ccf_rms_norm_backward_workspace_bytes(rows, d), total) if want_weight else None
+        _lib.call("ccf_rms_norm_backward", _ptr(grad_y), _ptr(total), _ptr(weight), _ptr(rstd), _ptr(grad_total), rows, d, code,
+                  _TYPE_CODES[weight.dtype], _ptr(g_x), _ptr(g_w), _ptr(ws), ws.numel() if want_weight else 0, _stream(total))
+    return g_x, g_w
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes [..., k] float8_e4m3fn, scale [..., ceil(k / 128)] float32) of rows in fp16, bf16 or fp32: for each row and 128
+    columns the least power of two that leaves no element beyond 448."""
+    _check(x, "x")
+    code = _type_code(x, "x")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("quantize_rows: x has no columns")
+    k = x.shape[-1]
+    codes = torch.empty(x.shape, dtype=FP8, device=x.device)
+    scale = torch.empty(*x.shape[:-1], _scale_blocks(k), dtype=torch.float32, device=x.device)
+    with _on(x):
+        _lib.call("ccf_quantize_rows", _ptr(x), x.numel() // k, k, code, _ptr(codes), _ptr(scale), _stream(x))
+    return codes, scale
+
+
+def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scale) of a weight [n, k] or [E, n, k] in fp16, bf16 or fp32: a scale for each block of 128 x 128,
+    [ceil(n / 128), ceil(k / 128)] with E in front where the weight has it."""
+    _check(w, "weight")
+    code = _type_code(w, "weight")
+    if w.dim() not in (2, 3) or w.shape[-1] == 0 or w.shape[-2] == 0:
+        raise ValueError(f"weight must be [n, k] or [E, n, k], got {tuple(w.shape)}")
+    n, k = w.shape[-2:]
+    E = w.shape[0] if w.dim() == 3 else 1
+    codes = torch.empty(w.shape, dtype=FP8, device=w.device)
+    scale = torch.empty(*w.shape[:-2], _scale_blocks(n), _scale_blocks(k), dtype=torch.float32, device=w.device)
+    with _on(w):
+        _lib.call("ccf_quantize_weight", _ptr(w), E, n, k, code, _ptr(codes), _ptr(scale), _stream(w))
+    return codes, scale

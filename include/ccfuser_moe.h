@@ -44,7 +44,7 @@ enum {
   CCF_ERR_UNSUPPORTED = 5  /* dtype or option not implemented                  */
 };
 
-enum { CCF_F16 = 0, CCF_F32 = 1 };
+enum { CCF_F16 = 0, CCF_F32 = 1, CCF_BF16 = 2 };
 
 /* Library version (major*10000 + minor*100 + patch). */
 int ccf_version(void);
@@ -595,6 +595,48 @@ int ccf_ffn_backward_pair(const void *grad_y_flat, const void *x, const void *ac
                           int d_model, int d_ffn, const void *w1, const void *w2, void *grad_x, void *grad_w1,
                           void *grad_b1, void *grad_w2, void *grad_b2, void *workspace, size_t workspace_bytes,
                           ccf_stream_t stream);
+
+/* --------------------------------------------------- norm and 8-bit rows */
+
+/*
+ * Root-mean-square norm of the rows of a residual stream (no counterpart in the reference, whose examples take their norms
+ * from torch):
+ *   total = x + residual, rounded to the rows' type (residual NULL: total is x, and the argument total is NULL)
+ *   y     = total * rstd * weight,  rstd = 1 / sqrt(mean(total^2) + eps), fp32 arithmetic, one rounding
+ *   codes, scales  the same fp32 y in 8 bits, as ccf_quantize_rows makes them
+ *   x, residual, y, total [rows, d] in `dtype` (CCF_F16, CCF_BF16 or CCF_F32); weight [d] in weight_dtype, which is dtype or
+ *   CCF_F32.  y or codes may be NULL, not both; codes uint8 [rows, d] and scales float [rows, ceil(d / 128)] go together;
+ *   rstd float [rows] or NULL (the backward reads it).  Pointers are aligned to their elements.
+ */
+int ccf_rms_norm(const void *x, const void *residual, const void *weight, int rows, int d, float eps, int dtype,
+                 int weight_dtype, void *y, void *total, void *codes, float *scales, float *rstd, ccf_stream_t stream);
+
+/* Bytes of workspace ccf_rms_norm_backward needs when it returns the weight gradient (no counterpart in the reference). */
+size_t ccf_rms_norm_backward_workspace_bytes(int rows, int d);
+
+/*
+ * Backward of ccf_rms_norm (no counterpart in the reference):
+ *   grad_x      = grad_total + rstd (g - total rstd^2 mean(g total)),  g = grad_y * weight
+ *   grad_weight = sum over rows of grad_y total rstd
+ * fp32 sums in a fixed order.  grad_total (the gradient that reaches total by other ways) may be NULL; grad_x, in the rows'
+ * type, is the gradient of x and of the residual alike; grad_x or grad_weight (in weight_dtype) may be NULL, not both.
+ */
+int ccf_rms_norm_backward(const void *grad_y, const void *total, const void *weight, const float *rstd,
+                          const void *grad_total, int rows, int d, int dtype, int weight_dtype, void *grad_x,
+                          void *grad_weight, void *workspace, size_t workspace_bytes, ccf_stream_t stream);
+
+/*
+ * Rows [rows, k] in `dtype` to 8 bits (no counterpart in the reference, which computes in fp16): e4m3 codes uint8 [rows, k]
+ * and a scale for each block of 128 columns, float [rows, ceil(k / 128)]; element = code * scale.  A scale is the least
+ * power of two, 2^-126 at least, that leaves no element of its block beyond 448, so a code is one rounding to nearest even.
+ * NaN and infinities become NaN codes.
+ */
+int ccf_quantize_rows(const void *x, int rows, int k, int dtype, void *codes, float *scales, ccf_stream_t stream);
+
+/* The same for weights [num_expert, n, k] (no counterpart in the reference), with a scale for each block of 128 x 128:
+ * scales float [num_expert, ceil(n / 128), ceil(k / 128)]. */
+int ccf_quantize_weight(const void *w, int num_expert, int n, int k, int dtype, void *codes, float *scales,
+                        ccf_stream_t stream);
 
 #ifdef __cplusplus
 }
