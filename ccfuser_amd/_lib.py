@@ -71,6 +71,9 @@ SIGNATURES = {
     "ccf_rms_norm_backward": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
     "ccf_quantize_rows": (_i, [_p, _i, _i, _i, _p, _p, _p]),
     "ccf_quantize_weight": (_i, [_p, _i, _i, _i, _i, _p, _p, _p]),
+    "ccf_linear_fp8": (_i, [_p, _p, _i, _i, _p, _p, _i, _p, _i, _p, _p]),
+    "ccf_ffn1_fp8": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p]),
+    "ccf_ffn2_fp8": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p]),
 }
 
 

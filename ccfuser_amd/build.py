@@ -20,7 +20,7 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libccfuser_moe.so"
 PROBE_LIB = HERE / "libccfuser_probe.so"
 SOURCES = ["api.hip", "gate.hip", "route.hip", "rows.hip", "bwd.hip", "few.hip", "thin.hip", "ffn.hip",
-           "norm.hip"]
+           "norm.hip", "gemm8.hip"]
 PROBE_SOURCES = ["probe.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

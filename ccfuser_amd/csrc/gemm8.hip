@@ -1,0 +1,538 @@
+// Matrix product in e4m3 with a scale for each block of 128, dense or grouped by expert, for gfx950.
+//
+//   y[r, n] = sum over blocks b of sa[r, b] sb[n / 128, b] (sum over k in b of a[r, k] w[n, k]) + bias[n]
+//
+// v_mfma_f32_16x16x128_f8f6f4 contracts one block: its result, from zero, is scaled by a row's and a weight block's scale
+// and added to the sum in fp32, four fused multiply-adds for an instruction of 32 cycles.  Weights are the A operand, so a
+// lane holds four consecutive columns of one row: one scale per lane and 16 rows, and stores of four columns.  (The
+// instruction's own scales are powers of two per 32 elements; weights come with scales of any value.)  The order of K
+// inside a lane's 32 bytes is that of memory for both operands, which is all that a product needs.
+//
+// Two kernels.  gemm8_tile_kernel: tiles through LDS, for many rows: bound by the matrix cores.  gemm8_split_kernel: a
+// workgroup's wavefronts cut K among them and read straight from memory, for few rows or few tiles: bound by the weights'
+// bytes or by a chain of loads.
+#include "gemm8.h"
+#include "gelu.h"
+
+#include <type_traits>
+
+namespace ccf {
+namespace {
+
+__device__ const int4v kZeros16 = {0, 0, 0, 0};              // what lanes behind the end of K read
+
+__device__ __forceinline__ float4v mfma8(int8v a, int8v b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, float4v{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+}
+
+__device__ __forceinline__ int8v join(int4v lo, int4v hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+struct Tile {
+  int e, row0, rows, m, n;   // expert (-1: none), first sorted row, rows of the expert from it on, tile indices
+};
+
+// Tile `t` of the grouped product in tiles of BM rows: expert by expert, inside one in groups of 8 tiles of rows, columns
+// outside, so that neighbours share both operands.  The experts' tiles are counted 64 experts at a time.
+template <int BM>
+__device__ __forceinline__ Tile find_tile(const Gemm8Args &p, int pid, int grid, int n_tiles) {
+  const int lane = threadIdx.x & 63;
+  auto span = [&](int e, int &lo, int &hi) {
+    lo = hi = 0;
+    if (e < p.E) {
+      lo = p.offsets ? p.offsets[e] : 0;
+      hi = p.offsets ? p.offsets[e + 1] : p.max_rows;
+      lo = lo < p.max_rows ? lo : p.max_rows;
+      hi = hi < p.max_rows ? hi : p.max_rows;
+    }
+  };
+  int total = 0;
+  for (int e0 = 0; e0 < p.E; e0 += 64) {
+    int lo, hi;
+    span(e0 + lane, lo, hi);
+    int mt = hi > lo ? (hi - lo + BM - 1) / BM : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mt += __shfl_xor(mt, o);
+    total += mt;
+  }
+  total = __builtin_amdgcn_readfirstlane(total) * n_tiles;
+  // workgroup ids go round the 8 XCDs: each XCD takes a run of tiles, which share operands in its L2
+  const int per = (total + 7) / 8;
+  int t = (pid & 7) * per + (pid >> 3);
+  Tile r{-1, 0, 0, 0, 0};
+  if ((pid >> 3) >= per || t >= total) return r;
+  int before = 0;
+  for (int e0 = 0; e0 < p.E; e0 += 64) {
+    int lo, hi;
+    span(e0 + lane, lo, hi);
+    const int mt = hi > lo ? (hi - lo + BM - 1) / BM : 0;
+    int upto = mt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o);
+      upto += lane >= o ? v : 0;
+    }
+    const unsigned long long past = __ballot((before + upto) * n_tiles > t);
+    if (past) {
+      const int who = __ffsll(past) - 1;
+      const int mts = __builtin_amdgcn_readlane(mt, who);
+      t -= (before + __builtin_amdgcn_readlane(upto, who) - mts) * n_tiles;
+      const int group = t / (8 * n_tiles), in = t - group * 8 * n_tiles;
+      const int gm = mts - group * 8 < 8 ? mts - group * 8 : 8;
+      r.e = e0 + who;
+      r.n = in / gm;
+      r.m = group * 8 + in - r.n * gm;
+      r.row0 = __builtin_amdgcn_readlane(lo, who) + r.m * BM;
+      r.rows = __builtin_amdgcn_readlane(hi, who) - r.row0;
+      return r;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return r;
+}
+
+// ------------------------------------------------------------------ tiles through LDS
+//
+// BM rows x BN columns, WM x WN wavefronts; a K step is a block of 128, staged by direct loads into one of two LDS places
+// while the other is multiplied.  16-byte chunks of a row lie at chunk ^ (row % 8), which the loads' global addresses
+// apply: eight lanes that read one chunk of eight rows take different banks.
+template <int BM, int BN, int WM, int WN>
+struct TileShape {
+  static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
+  static constexpr int TT = BM / WM / 16, CT = BN / WN / 16;       // 16 x 16 products of a wavefront: rows, columns
+  static constexpr int kStage = (BM + BN) * kScaleBlock;           // bytes
+  static constexpr int kLoadsX = BM / 8 / kWaves, kLoadsW = BN / 8 / kWaves;      // loads of 1 KB per wavefront and step
+};
+
+__device__ __forceinline__ void load_to_lds(const uint8_t *src, char *dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                   (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+
+// One K step: the loads of the next one into `next` (restrict: not what is read here, so nothing waits for them), then the
+// products of `now`.
+template <class S>
+__device__ __forceinline__ void tile_step(char *__restrict__ next, const char *__restrict__ now, bool more,
+                                          const uint8_t *const (&src)[S::kLoadsX + S::kLoadsW], int wave, int x_at, int w_at,
+                                          const float (&s)[S::TT], float4v (&acc)[S::CT][S::TT]) {
+  if (more) {
+#pragma unroll
+    for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i)
+      load_to_lds(src[i], next + (i * S::kWaves + wave) * 1024);
+  }
+  int8v x[S::TT];
+#pragma unroll
+  for (int t = 0; t < S::TT; ++t) {
+    const char *q = now + x_at + t * 16 * kScaleBlock;
+    x[t] = join(*reinterpret_cast<const int4v *>(q), *reinterpret_cast<const int4v *>(now + (x_at ^ 16) + t * 16 * kScaleBlock));
+  }
+#pragma unroll
+  for (int c = 0; c < S::CT; ++c) {
+    const int8v w = join(*reinterpret_cast<const int4v *>(now + w_at + c * 16 * kScaleBlock),
+                         *reinterpret_cast<const int4v *>(now + (w_at ^ 16) + c * 16 * kScaleBlock));
+    float4v part[S::TT];
+#pragma unroll
+    for (int t = 0; t < S::TT; ++t) part[t] = mfma8(w, x[t]);
+#pragma unroll
+    for (int t = 0; t < S::TT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[c][t][i] = fmaf(part[t][i], s[t], acc[c][t][i]);
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int kOut>
+__global__ void __launch_bounds__(WM * WN * 64, 2)
+gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
+  using S = TileShape<BM, BN, WM, WN>;
+  using Out = std::conditional_t<kOut == kGemm8Bf16, bf16_t, half_t>;
+  extern __shared__ __attribute__((aligned(1024))) char s_tile[];
+  const Tile tile = find_tile<BM>(p, blockIdx.x, gridDim.x, n_tiles);
+  if (tile.e < 0) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int wm = wave / WN, wn = wave % WN;
+  const int KB = scale_blocks(p.K), NB = scale_blocks(p.N), tail = p.K % kScaleBlock;
+  const int rows = tile.rows < BM ? tile.rows : BM, n0 = tile.n * BN;
+  auto a_row = [&](int r) {                          // past the end: the last row again, never stored
+    const int j = tile.row0 + (r < rows ? r : rows - 1);
+    return static_cast<size_t>(p.a_rows ? p.a_rows[j] : j);
+  };
+
+  // sources of this lane's loads: row i * 8 * waves + 8 * wave + lane / 8 of the stage, chunk (lane % 8) ^ (row % 8)
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  const uint8_t *src[S::kLoadsX + S::kLoadsW];
+#pragma unroll
+  for (int i = 0; i < S::kLoadsX; ++i)
+    src[i] = p.a + a_row((i * S::kWaves + wave) * 8 + (lane >> 3)) * p.K + chunk * 16;
+  const uint8_t *w_e = p.b + static_cast<size_t>(tile.e) * p.N * p.K;
+#pragma unroll
+  for (int i = 0; i < S::kLoadsW; ++i) {
+    const int n = n0 + (i * S::kWaves + wave) * 8 + (lane >> 3);
+    src[S::kLoadsX + i] = w_e + static_cast<size_t>(n < p.N ? n : p.N - 1) * p.K + chunk * 16;
+  }
+  const float *sa[S::TT];
+#pragma unroll
+  for (int t = 0; t < S::TT; ++t) sa[t] = p.a_scale + a_row(wm * (BM / WM) + t * 16 + r16) * KB;
+  int nb = (n0 + wn * (BN / WN)) / kScaleBlock;       // a wavefront's columns share it
+  nb = nb < NB ? nb : NB - 1;
+  const float *sb = p.b_scale + (static_cast<size_t>(tile.e) * NB + nb) * KB;
+
+  auto next_sources = [&](int kb) {                   // sources of step kb, from those of kb - 1
+#pragma unroll
+    for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i) src[i] += kScaleBlock;
+    if (tail && kb == KB - 1 && chunk * 16 >= tail) {
+#pragma unroll
+      for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i) src[i] = reinterpret_cast<const uint8_t *>(&kZeros16);
+    }
+  };
+  auto scales = [&](int kb, float (&s)[S::TT]) {
+    const float b = sb[kb];
+#pragma unroll
+    for (int t = 0; t < S::TT; ++t) s[t] = sa[t][kb] * b;
+  };
+
+  float4v acc[S::CT][S::TT];
+#pragma unroll
+  for (int c = 0; c < S::CT; ++c)
+#pragma unroll
+    for (int t = 0; t < S::TT; ++t) acc[c][t] = float4v{0, 0, 0, 0};
+  const int x_at = (wm * (BM / WM) + r16) * kScaleBlock + ((2 * g) ^ (r16 & 7)) * 16;
+  const int w_at = (BM + wn * (BN / WN) + r16) * kScaleBlock + ((2 * g) ^ (r16 & 7)) * 16;
+
+  if (KB == 1 && tail && chunk * 16 >= tail) {
+#pragma unroll
+    for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i) src[i] = reinterpret_cast<const uint8_t *>(&kZeros16);
+  }
+#pragma unroll
+  for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i) load_to_lds(src[i], s_tile + (i * S::kWaves + wave) * 1024);
+  float s[S::TT], s_next[S::TT];
+  scales(0, s);
+  int place = 0;
+  for (int kb = 0; kb < KB; ++kb) {
+    // this step's loads have landed and every wavefront is done with the place that the next step's go to
+    __builtin_amdgcn_s_waitcnt(0x0f70);               // vmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const bool more = kb + 1 < KB;
+    if (more) {
+      next_sources(kb + 1);
+      scales(kb + 1, s_next);
+    }
+    tile_step<S>(s_tile + (place ^ 1) * S::kStage, s_tile + place * S::kStage, more, src, wave, x_at, w_at, s, acc);
+    place ^= 1;
+#pragma unroll
+    for (int t = 0; t < S::TT; ++t) s[t] = s_next[t];
+  }
+
+  // a lane holds one row and, in every product, four consecutive columns
+  const Out *bias = p.bias ? static_cast<const Out *>(p.bias) + static_cast<size_t>(tile.e) * p.N : nullptr;
+  const int col0 = n0 + wn * (BN / WN) + 4 * g;
+#pragma unroll
+  for (int t = 0; t < S::TT; ++t) {
+    const int r = wm * (BM / WM) + t * 16 + r16;
+    const bool mine = r < rows;
+    const int j = tile.row0 + (mine ? r : 0);
+    const size_t crow = static_cast<size_t>(p.c_rows && mine ? p.c_rows[j] : j);
+    if constexpr (kOut == kGemm8Gelu8) {
+      float top = 0.0f;
+#pragma unroll
+      for (int c = 0; c < S::CT; ++c) {
+        const int col = col0 + 16 * c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float b = bias && col < p.N ? static_cast<float>(bias[col + i]) : 0.0f;
+          const float v = col < p.N ? gelu_erf(acc[c][t][i] + b) : 0.0f;
+          acc[c][t][i] = v;
+          top = fmaxf(top, fabsf(v));
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      float inverse;
+      const float scale = block_scale(top, &inverse);
+      if (mine && col0 < p.N) {
+        if (g == 0) p.scales[crow * NB + nb] = scale;
+#pragma unroll
+        for (int c = 0; c < S::CT; ++c)
+          if (col0 + 16 * c < p.N)
+            *reinterpret_cast<int *>(p.codes + crow * p.N + col0 + 16 * c) =
+                pack_fp8(acc[c][t][0] * inverse, acc[c][t][1] * inverse, acc[c][t][2] * inverse, acc[c][t][3] * inverse);
+      }
+    } else if (mine) {
+      typedef Out out4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int c = 0; c < S::CT; ++c) {
+        const int col = col0 + 16 * c;
+        if (col >= p.N) continue;
+        out4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = static_cast<Out>(acc[c][t][i] + (bias ? static_cast<float>(bias[col + i]) : 0.0f));
+        *reinterpret_cast<out4 *>(static_cast<Out *>(p.c) + crow * p.N + col) = o;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------- K cut over the wavefronts of a workgroup
+//
+// 16 TT rows x 16 CT CS columns; KS = 8 / CS wavefronts take every KS-th block of K each, straight from memory, and their
+// sums meet in LDS.  Two blocks are on their way while one is multiplied.
+template <int TT, int CT, int CS>
+struct SplitShape {
+  static constexpr int kWaves = 8, KS = kWaves / CS, BM = 16 * TT, BN = 16 * CT * CS, kLd = BN + 4;
+  static constexpr size_t kLds = sizeof(float) * KS * BM * kLd;
+};
+
+template <int TT, int CT, int CS, int kOut>
+__global__ void __launch_bounds__(512, 2)
+gemm8_split_kernel(Gemm8Args p, int n_tiles) {
+  using S = SplitShape<TT, CT, CS>;
+  using Out = std::conditional_t<kOut == kGemm8Bf16, bf16_t, half_t>;
+  extern __shared__ __attribute__((aligned(16))) float s_part[];           // [KS][BM][kLd]
+  const Tile tile = find_tile<S::BM>(p, blockIdx.x, gridDim.x, n_tiles);
+  if (tile.e < 0) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4, ks = wave % S::KS, cs = wave / S::KS;
+  const int KB = scale_blocks(p.K), NB = scale_blocks(p.N);
+  const int rows = tile.rows < S::BM ? tile.rows : S::BM, n0 = tile.n * S::BN, c0 = n0 + cs * 16 * CT;
+  const uint8_t *x[TT];
+  const float *sa[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int r = 16 * t + r16, j = tile.row0 + (r < rows ? r : rows - 1);
+    const size_t row = static_cast<size_t>(p.a_rows ? p.a_rows[j] : j);
+    x[t] = p.a + row * p.K + 32 * g;
+    sa[t] = p.a_scale + row * KB;
+  }
+  const uint8_t *w[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int n = c0 + 16 * c + r16;
+    w[c] = p.b + (static_cast<size_t>(tile.e) * p.N + (n < p.N ? n : p.N - 1)) * p.K + 32 * g;
+  }
+  int nb = c0 / kScaleBlock;
+  nb = nb < NB ? nb : NB - 1;
+  const float *sb = p.b_scale + (static_cast<size_t>(tile.e) * NB + nb) * KB;
+  float4v acc[CT][TT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[c][t] = float4v{0, 0, 0, 0};
+
+  const int count = KB > ks ? (KB - ks + S::KS - 1) / S::KS : 0;           // blocks ks, ks + KS, ...
+  int8v wf[2][CT], xf[2][TT];
+  float sf[2][TT];
+  auto piece = [&](const uint8_t *q, int kb) {
+    const uint8_t *at = q + static_cast<size_t>(kb) * kScaleBlock;
+    const int left = p.K - kb * kScaleBlock - 32 * g;                      // codes of the row from this lane's first on
+    const int4v *lo = reinterpret_cast<const int4v *>(left > 0 ? at : reinterpret_cast<const uint8_t *>(&kZeros16));
+    const int4v *hi = reinterpret_cast<const int4v *>(left > 16 ? at + 16 : reinterpret_cast<const uint8_t *>(&kZeros16));
+    return join(*lo, *hi);
+  };
+  auto whole = [&](const uint8_t *q, int kb) {
+    const int4v *at = reinterpret_cast<const int4v *>(q + static_cast<size_t>(kb) * kScaleBlock);
+    return join(at[0], at[1]);
+  };
+  auto fetch = [&](int i, auto B_) {                                       // the wavefront's block i; past the last one it again
+    constexpr int buf = decltype(B_)::value;
+    const int kb = ks + (i < count ? i : count - 1) * S::KS;
+    const float b = sb[kb];
+    if ((kb + 1) * kScaleBlock <= p.K) {                                   // uniform
+#pragma unroll
+      for (int c = 0; c < CT; ++c) wf[buf][c] = whole(w[c], kb);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) xf[buf][t] = whole(x[t], kb);
+    } else {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) wf[buf][c] = piece(w[c], kb);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) xf[buf][t] = piece(x[t], kb);
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) sf[buf][t] = sa[t][kb] * b;
+  };
+  auto multiply = [&](int i, auto B_) {
+    constexpr int buf = decltype(B_)::value;
+    if (i >= count) return;                                                // uniform
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      float4v part[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) part[t] = mfma8(wf[buf][c], xf[buf][t]);
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[c][t][q] = fmaf(part[t][q], sf[buf][t], acc[c][t][q]);
+    }
+  };
+  if (count > 0) {
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    fetch(0, even);
+    for (int i = 0; i < count; i += 2) {
+      fetch(i + 1, odd);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(i, even);
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(i + 2, even);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(i + 1, odd);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+      *reinterpret_cast<float4v *>(s_part + (ks * S::BM + 16 * t + r16) * S::kLd + (cs * CT + c) * 16 + 4 * g) = acc[c][t];
+  __syncthreads();
+  // eight consecutive columns to a thread, 16 threads to a scale's block
+  const Out *bias = p.bias ? static_cast<const Out *>(p.bias) + static_cast<size_t>(tile.e) * p.N : nullptr;
+  constexpr int kPer = S::BN / 8;
+  for (int i = threadIdx.x; i < S::BM * kPer; i += 512) {
+    const int r = i / kPer, c = (i % kPer) * 8, col = n0 + c;
+    const bool mine = r < rows && col < p.N;
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < S::KS; ++k) {
+      const float *part = s_part + (k * S::BM + r) * S::kLd + c;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += part[q];
+    }
+    if (bias && mine) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += static_cast<float>(bias[col + q]);
+    }
+    const int j = tile.row0 + r;
+    const size_t crow = mine && p.c_rows ? static_cast<size_t>(p.c_rows[j]) : static_cast<size_t>(j);
+    if constexpr (kOut == kGemm8Gelu8) {
+      float top = 0.0f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        v[q] = mine ? gelu_erf(v[q]) : 0.0f;
+        top = fmaxf(top, fabsf(v[q]));
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+      float inverse;
+      const float scale = block_scale(top, &inverse);
+      if (mine) {
+        if ((i & 15) == 0) p.scales[crow * NB + col / kScaleBlock] = scale;
+        *reinterpret_cast<int2v *>(p.codes + crow * p.N + col) =
+            int2v{pack_fp8(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
+                  pack_fp8(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse)};
+      }
+    } else if (mine) {
+      typedef Out out8 __attribute__((ext_vector_type(8)));
+      out8 o;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) o[q] = static_cast<Out>(v[q]);
+      *reinterpret_cast<out8 *>(static_cast<Out *>(p.c) + crow * p.N + col) = o;
+    }
+  }
+}
+
+// Workgroups: every tile that the rows may make, in whole rounds of the XCDs.
+long long grid_of(const Gemm8Args &p, int bm, int n_tiles) {
+  const long long m = p.max_rows / bm + (p.offsets ? (p.E < p.max_rows ? p.E : p.max_rows) : 1);
+  return (m * n_tiles + 7) / 8 * 8;
+}
+
+template <typename K>
+int launch(K kernel, const Gemm8Args &p, int bm, int bn, int threads, size_t lds, hipStream_t st, const char *what) {
+  const int n_tiles = (p.N + bn - 1) / bn;
+  const long long grid = grid_of(p, bm, n_tiles);
+  CCF_REQUIRE(grid < (1ll << 28), CCF_ERR_SHAPE, "%s: too many tiles", what);
+  if (lds > 65536) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(lds));
+    if (e != hipSuccess) return fail(CCF_ERR_HIP, "%s: LDS attribute: %s", what, hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), lds, st, p, n_tiles);
+  return check_launch(what);
+}
+
+template <int BM, int BN, int WM, int WN, int kOut>
+int launch_tiles(const Gemm8Args &p, hipStream_t st, const char *what) {
+  using S = TileShape<BM, BN, WM, WN>;
+  return launch(gemm8_tile_kernel<BM, BN, WM, WN, kOut>, p, BM, BN, S::kThreads, 2 * S::kStage, st, what);
+}
+
+template <int TT, int CT, int CS, int kOut>
+int launch_split(const Gemm8Args &p, hipStream_t st, const char *what) {
+  using S = SplitShape<TT, CT, CS>;
+  return launch(gemm8_split_kernel<TT, CT, CS, kOut>, p, S::BM, S::BN, 512, S::kLds, st, what);
+}
+
+template <int kOut>
+int gemm8_out(const Gemm8Args &p, hipStream_t st, const char *what) {
+  const int owners = p.offsets ? (p.E < p.max_rows ? p.E : p.max_rows) : 1;
+  const int rows = (p.max_rows + owners - 1) / owners;         // of an expert, loads being even
+  // (the 8-bit output wants all 128 columns of a scale in one workgroup)
+  constexpr int CS = kOut == kGemm8Gelu8 ? 2 : 1;
+  if (rows <= 16) return launch_split<1, 4, CS, kOut>(p, st, what);
+  if (rows <= 32) return launch_split<2, 4, CS, kOut>(p, st, what);
+  const long long large = static_cast<long long>(p.max_rows / 256 + owners) * ((p.N + 255) / 256);
+  if (rows <= 128 || large < 256) return launch_split<4, 4, 2, kOut>(p, st, what);
+  return launch_tiles<256, 256, 4, 2, kOut>(p, st, what);
+}
+
+}  // namespace
+
+int gemm8(const Gemm8Args &p, int out, hipStream_t st, const char *what) {
+  if (p.max_rows == 0 || p.E == 0) return CCF_OK;
+  if (out == kGemm8Half) return gemm8_out<kGemm8Half>(p, st, what);
+  if (out == kGemm8Bf16) return gemm8_out<kGemm8Bf16>(p, st, what);
+  return gemm8_out<kGemm8Gelu8>(p, st, what);
+}
+
+namespace {
+
+int check_product(const Gemm8Args &p, const char *what) {
+  CCF_REQUIRE(p.max_rows >= 0 && p.E > 0 && p.N > 0 && p.K > 0, CCF_ERR_ARG, "%s: bad size", what);
+  CCF_REQUIRE(p.E <= 1024, CCF_ERR_SHAPE, "%s: num_expert=%d beyond 1024", what, p.E);
+  CCF_REQUIRE(p.K % 16 == 0 && p.N % 8 == 0, CCF_ERR_SHAPE, "%s: contraction of %d and %d columns: multiples of 16 and 8 are needed",
+              what, p.K, p.N);
+  if (p.max_rows == 0) return CCF_OK;
+  CCF_REQUIRE(p.a && p.a_scale && p.b && p.b_scale && (p.c || (p.codes && p.scales)), CCF_ERR_ARG, "%s: null pointer", what);
+  CCF_REQUIRE(aligned16(p.a) && aligned16(p.b) && aligned16(p.c) && aligned16(p.codes) && aligned16(p.bias), CCF_ERR_ARG,
+              "%s: rows must be 16-byte aligned", what);
+  return CCF_OK;
+}
+
+}  // namespace
+}  // namespace ccf
+
+extern "C" int ccf_linear_fp8(const void *x_codes, const float *x_scales, int rows, int k, const void *w_codes,
+                              const float *w_scales, int n, const void *bias, int dtype, void *y, ccf_stream_t stream) {
+  using namespace ccf;
+  CCF_REQUIRE(dtype == CCF_F16 || dtype == CCF_BF16, CCF_ERR_UNSUPPORTED, "linear_fp8: output of type %d", dtype);
+  const Gemm8Args p{static_cast<const uint8_t *>(x_codes), x_scales, nullptr, static_cast<const uint8_t *>(w_codes), w_scales, bias,
+                    nullptr, rows, 1, n, k, nullptr, y, nullptr, nullptr};
+  if (int rc = check_product(p, "linear_fp8")) return rc;
+  return gemm8(p, dtype == CCF_F16 ? kGemm8Half : kGemm8Bf16, as_stream(stream), "linear_fp8");
+}
+
+extern "C" int ccf_ffn1_fp8(const void *x_codes, const float *x_scales, const int32_t *src_row, const int32_t *offsets, int max_rows,
+                            int num_expert, int d_model, int d_ffn, const void *w1_codes, const float *w1_scales, const void *b1,
+                            void *h_codes, float *h_scales, ccf_stream_t stream) {
+  using namespace ccf;
+  const Gemm8Args p{static_cast<const uint8_t *>(x_codes), x_scales, src_row, static_cast<const uint8_t *>(w1_codes), w1_scales, b1,
+                    offsets, max_rows, num_expert, d_ffn, d_model, nullptr, nullptr, static_cast<uint8_t *>(h_codes), h_scales};
+  if (int rc = check_product(p, "ffn1_fp8")) return rc;
+  CCF_REQUIRE(offsets || max_rows == 0, CCF_ERR_ARG, "ffn1_fp8: null pointer");
+  return gemm8(p, kGemm8Gelu8, as_stream(stream), "ffn1_fp8");
+}
+
+extern "C" int ccf_ffn2_fp8(const void *h_codes, const float *h_scales, const int32_t *dst_row, const int32_t *offsets, int max_rows,
+                            int num_expert, int d_model, int d_ffn, const void *w2_codes, const float *w2_scales, const void *b2,
+                            void *y, ccf_stream_t stream) {
+  using namespace ccf;
+  const Gemm8Args p{static_cast<const uint8_t *>(h_codes), h_scales, nullptr, static_cast<const uint8_t *>(w2_codes), w2_scales, b2,
+                    offsets, max_rows, num_expert, d_model, d_ffn, dst_row, y, nullptr, nullptr};
+  if (int rc = check_product(p, "ffn2_fp8")) return rc;
+  CCF_REQUIRE(offsets || max_rows == 0, CCF_ERR_ARG, "ffn2_fp8: null pointer");
+  return gemm8(p, kGemm8Half, as_stream(stream), "ffn2_fp8");
+}

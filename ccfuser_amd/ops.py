@@ -846,3 +846,113 @@ def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     with _on(w):
         _lib.call("ccf_quantize_weight", _ptr(w), E, n, k, code, _ptr(codes), _ptr(scale), _stream(w))
     return codes, scale
+
+
+# ------------------------------------------------------- products in 8 bits
+def _check_fp8(codes: torch.Tensor, scale: torch.Tensor, name: str, block_rows: bool, ndim: int) -> None:
+    """Codes [..., n, k] and their scales: one per row (or per 128 rows) and 128 columns."""
+    _check(codes, f"{name} codes", dtype=FP8, ndim=ndim)
+    _check(scale, f"{name} scale", dtype=torch.float32, ndim=ndim)
+    n, k = codes.shape[-2:]
+    want = (*codes.shape[:-2], _scale_blocks(n) if block_rows else n, _scale_blocks(k))
+    if tuple(scale.shape) != want:
+        raise ValueError(f"{name}: scale {tuple(scale.shape)} does not match codes {tuple(codes.shape)}, expected {want}")
+    _same_device(codes, scale)
+
+
+def _rows_fp8(x, name: str):
+    """(codes, scale) of rows [r, k] that are given in 8 bits, as such a pair, or in 16 or 32, and are quantised here."""
+    if isinstance(x, torch.Tensor):
+        _check(x, name, ndim=2)
+        return quantize_rows(x)
+    codes, scale = x
+    _check_fp8(codes, scale, name, False, 2)
+    return codes, scale
+
+
+def linear_fp8(x, w_codes: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x @ w.T + bias`` in 8 bits: y [r, n] in ``dtype``, float16 or bfloat16.  ``x`` is [r, k] in fp16 or bf16 (quantised by
+    the call; ``dtype`` is x's unless given) or a pair as ``quantize_rows`` returns it (float16 unless given); the weight is
+    [n, k] as ``quantize_weight`` returns it, or any codes with any scale per 128 x 128 block; ``bias`` [n] has y's type.
+    k is a multiple of 16, n of 8.  Not differentiable: weights in 8 bits are for serving."""
+    if isinstance(x, torch.Tensor) and dtype is None:
+        dtype = x.dtype
+    dtype = torch.float16 if dtype is None else dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"linear_fp8 returns float16 or bfloat16, not {dtype}")
+    codes, scale = _rows_fp8(x, "x")
+    _check_fp8(w_codes, w_scale, "weight", True, 2)
+    rows, k = codes.shape
+    n = w_codes.shape[0]
+    if w_codes.shape[1] != k:
+        raise ValueError(f"linear_fp8: x {tuple(codes.shape)} and weight {tuple(w_codes.shape)} do not match")
+    if bias is not None:
+        _check(bias, "bias", dtype=dtype, ndim=1)
+        if bias.shape[0] != n:
+            raise ValueError("linear_fp8: bias and weight do not match")
+    _same_device(codes, w_codes, bias)
+    y = torch.empty(rows, n, dtype=dtype, device=codes.device)
+    with _on(codes):
+        _lib.call("ccf_linear_fp8", _ptr(codes), _ptr(scale), rows, k, _ptr(w_codes), _ptr(w_scale), n, _ptr(bias),
+                  _TYPE_CODES[dtype], _ptr(y), _stream(codes))
+    return y
+
+
+def _check_expert_fp8(codes, scale, bias, name: str) -> None:
+    _check_fp8(codes, scale, name, True, 3)
+    if bias is not None:
+        _check(bias, f"{name} bias", dtype=torch.float16, ndim=2)
+        if tuple(bias.shape) != tuple(codes.shape[:2]):
+            raise ValueError(f"{name}: bias {tuple(bias.shape)} does not match weight {tuple(codes.shape)}")
+        _same_device(codes, bias)
+
+
+def ffn1_fp8(x, src_row: Optional[torch.Tensor], offsets: torch.Tensor, max_rows: int, w1_codes: torch.Tensor,
+             w1_scale: torch.Tensor, b1: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes [max_rows, f], scale [max_rows, ceil(f / 128)]): ``ffn1`` with the GELU, in 8 bits throughout.  ``x`` is [T, d]
+    in 16 bits or a pair as ``quantize_rows`` returns it, the weight [E, f, d] in 8 bits.  Rows nothing maps to are
+    undefined."""
+    codes, scale = _rows_fp8(x, "x")
+    _check_expert_fp8(w1_codes, w1_scale, b1, "ffn1")
+    _check(offsets, "offsets", dtype=torch.int32, ndim=1)
+    E, f, d = w1_codes.shape
+    if codes.shape[1] != d or offsets.numel() != E + 1:
+        raise ValueError("ffn1_fp8: x/offsets do not match the weight shape")
+    if src_row is not None:
+        _check(src_row, "src_row", dtype=torch.int32, ndim=1)
+        if src_row.numel() < max_rows:
+            raise ValueError("ffn1_fp8: src_row shorter than max_rows")
+    elif codes.shape[0] < max_rows:
+        raise ValueError("ffn1_fp8: x has fewer rows than max_rows")
+    _same_device(codes, src_row, offsets, w1_codes)
+    h = torch.empty(max_rows, f, dtype=FP8, device=codes.device)
+    h_scale = torch.empty(max_rows, _scale_blocks(f), dtype=torch.float32, device=codes.device)
+    with _on(codes):
+        _lib.call("ccf_ffn1_fp8", _ptr(codes), _ptr(scale), _ptr(src_row), _ptr(offsets), int(max_rows), E, d, f, _ptr(w1_codes),
+                  _ptr(w1_scale), _ptr(b1), _ptr(h), _ptr(h_scale), _stream(codes))
+    return h, h_scale
+
+
+def ffn2_fp8(h, dst_row: Optional[torch.Tensor], offsets: torch.Tensor, max_rows: int, w2_codes: torch.Tensor,
+             w2_scale: torch.Tensor, b2: Optional[torch.Tensor], y: torch.Tensor) -> torch.Tensor:
+    """Writes ``y[dst_row[j]]`` (fp16) for the routed rows and returns ``y``: ``ffn2`` in 8 bits.  ``h`` is what ``ffn1_fp8``
+    returns, or rows in 16 bits; the weight [E, d, f] in 8 bits."""
+    codes, scale = _rows_fp8(h, "h")
+    _check_expert_fp8(w2_codes, w2_scale, b2, "ffn2")
+    _check(offsets, "offsets", dtype=torch.int32, ndim=1)
+    _check(y, "y", dtype=torch.float16, ndim=2)
+    E, d, f = w2_codes.shape
+    if codes.shape[1] != f or offsets.numel() != E + 1 or y.shape[1] != d or codes.shape[0] < max_rows:
+        raise ValueError("ffn2_fp8: h/offsets/y do not match the weight shape")
+    if dst_row is not None:
+        _check(dst_row, "dst_row", dtype=torch.int32, ndim=1)
+        if dst_row.numel() < max_rows:
+            raise ValueError("ffn2_fp8: dst_row shorter than max_rows")
+    elif y.shape[0] < max_rows:
+        raise ValueError("ffn2_fp8: y has fewer rows than max_rows")
+    _same_device(codes, dst_row, offsets, w2_codes, y)
+    with _on(codes):
+        _lib.call("ccf_ffn2_fp8", _ptr(codes), _ptr(scale), _ptr(dst_row), _ptr(offsets), int(max_rows), E, d, f, _ptr(w2_codes),
+                  _ptr(w2_scale), _ptr(b2), _ptr(y), _stream(codes))
+    return y

@@ -638,6 +638,35 @@ int ccf_quantize_rows(const void *x, int rows, int k, int dtype, void *codes, fl
 int ccf_quantize_weight(const void *w, int num_expert, int n, int k, int dtype, void *codes, float *scales,
                         ccf_stream_t stream);
 
+/*
+ * Dense product in 8 bits (no counterpart in the reference, which computes in fp16):
+ *   y[r, j] = sum over blocks b of x_scales[r, b] w_scales[j / 128, b] (sum over k in b of x_codes[r, k] w_codes[j, k]) + bias[j]
+ *   x_codes [rows, k] and x_scales [rows, ceil(k / 128)] as ccf_quantize_rows leaves them, w_codes [n, k] and w_scales
+ *   [ceil(n / 128), ceil(k / 128)] as ccf_quantize_weight does; scales may have any finite value.  bias [n] or NULL and y
+ *   [rows, n] in dtype, CCF_F16 or CCF_BF16.  fp32 accumulation, one rounding.  k % 16 == 0, n % 8 == 0; codes, bias and y
+ *   16-byte aligned.
+ */
+int ccf_linear_fp8(const void *x_codes, const float *x_scales, int rows, int k, const void *w_codes, const float *w_scales,
+                   int n, const void *bias, int dtype, void *y, ccf_stream_t stream);
+
+/*
+ * ccf_ffn1_forward in 8 bits: h = gelu(x[src_row[j], :] * w1[e]^T + b1[e]) for offsets[e] <= j < offsets[e+1], left as codes
+ * [max_rows, d_ffn] and scales [max_rows, ceil(d_ffn / 128)] of the fp32 value, in expert order.  src_row NULL means row j;
+ * w1 codes [E, d_ffn, d_model] with scales per 128 x 128 block, b1 fp16 [E, d_ffn] or NULL.  Rows from offsets[E] on are left
+ * as they were.  (mix_moe/csrc/mix_moe.h:236-298 in fp16.)
+ */
+int ccf_ffn1_fp8(const void *x_codes, const float *x_scales, const int32_t *src_row, const int32_t *offsets, int max_rows,
+                 int num_expert, int d_model, int d_ffn, const void *w1_codes, const float *w1_scales, const void *b1,
+                 void *h_codes, float *h_scales, ccf_stream_t stream);
+
+/*
+ * ccf_ffn2_forward in 8 bits: y[dst_row[j], :] = h[j, :] * w2[e]^T + b2[e], fp16 (mix_moe/csrc/mix_moe.h:390-437 in fp16).
+ * dst_row NULL means row j; rows of y that no j maps to are left as they were.
+ */
+int ccf_ffn2_fp8(const void *h_codes, const float *h_scales, const int32_t *dst_row, const int32_t *offsets, int max_rows,
+                 int num_expert, int d_model, int d_ffn, const void *w2_codes, const float *w2_scales, const void *b2, void *y,
+                 ccf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
