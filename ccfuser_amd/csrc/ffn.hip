@@ -18,6 +18,7 @@
 #include "ccf_common.h"
 #include "gemm_tile.h"
 #include "gelu.h"
+#include "gemm8.h"
 #include "plan.h"
 
 #include <cmath>
@@ -1859,6 +1860,11 @@ extern "C" int ccf_set_option(const char *name, int value) {
     CCF_REQUIRE((value >= 0 && value <= 3) || (value >= 16 && value < 22), CCF_ERR_ARG,
                 "set_option: few_rows %d is neither 0..3 nor 16..21", value);
     g_few_rows = value;
+    return CCF_OK;
+  }
+  if (!strcmp(name, "fp8_form")) {           // products in 8 bits: 0 by the rule, 1 K cut over the wavefronts, 2 tiles in LDS
+    CCF_REQUIRE(value >= 0 && value <= 2, CCF_ERR_ARG, "set_option: fp8_form %d outside 0..2", value);
+    g_fp8_form = value;
     return CCF_OK;
   }
   if (!strcmp(name, "few_rows_places")) {

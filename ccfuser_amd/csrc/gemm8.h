@@ -22,6 +22,8 @@ struct Gemm8Args {
 
 enum { kGemm8Half = 0, kGemm8Bf16 = 1, kGemm8Gelu8 = 2 };     // the output: fp16, bf16, or GELU and 8 bits
 
+extern int g_fp8_form;       // ccf_set_option("fp8_form"): 0, 1 or 2
+
 int gemm8(const Gemm8Args &p, int out, hipStream_t stream, const char *what);
 
 int launch_quantize_rows(const void *x, int rows, int k, int dtype, uint8_t *codes, float *scales, hipStream_t st);

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 namespace ccf {
+int g_fp8_form = 0;          // 0: by the rule of gemm8_out; 1: K cut over the wavefronts always; 2: tiles through LDS always
 namespace {
 
 __device__ const int4v kZeros16 = {0, 0, 0, 0};              // what lanes behind the end of K read
@@ -94,49 +95,32 @@ __device__ __forceinline__ Tile find_tile(const Gemm8Args &p, int pid, int grid,
 //
 // BM rows x BN columns, WM x WN wavefronts; a K step is a block of 128, staged by direct loads into one of two LDS places
 // while the other is multiplied.  16-byte chunks of a row lie at chunk ^ (row % 8), which the loads' global addresses
-// apply: eight lanes that read one chunk of eight rows take different banks.
+// apply: eight lanes that read one chunk of eight rows take different banks.  The scales of a step come the same way, a
+// lane per row, and lie by row.
+//
+// A wavefront reads its rows' fragments once a step and its columns' one by one, two in turn.  The step's one barrier stands
+// in front of its last columns, whose fragment is in registers by then: behind it this step's place is free for the loads
+// of the step after the next, and the next step's rows are read between the last products, each into the registers that a
+// product has just let go.  So the matrix cores run through the steps, and a load has a whole step to land.
 template <int BM, int BN, int WM, int WN>
 struct TileShape {
   static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
   static constexpr int TT = BM / WM / 16, CT = BN / WN / 16;       // 16 x 16 products of a wavefront: rows, columns
-  static constexpr int kStage = (BM + BN) * kScaleBlock;           // bytes
+  static constexpr int kRowsBytes = (BM + BN) * kScaleBlock;       // a place: codes, then scales of rows, then of columns
+  static constexpr int kStage = kRowsBytes + 4 * (BM + 64);
   static constexpr int kLoadsX = BM / 8 / kWaves, kLoadsW = BN / 8 / kWaves;      // loads of 1 KB per wavefront and step
+  static constexpr int kLoads = kLoadsX + kLoadsW;
+  static_assert(kWaves >= BM / 64 + 1, "a wavefront more than the rows' scales take loads the columns'");
 };
 
-__device__ __forceinline__ void load_to_lds(const uint8_t *src, char *dst) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                   (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+// Direct loads to LDS at byte `at` + 16 (or 4) * lane.  In asm so that the compiler, which cannot tell the two places
+// apart, does not wait for them in front of every LDS read: they write no register, and the step's own wait and barrier
+// stand between them and any read of what they bring.
+__device__ __forceinline__ void load16_to_lds(const void *src, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src));
 }
-
-// One K step: the loads of the next one into `next` (restrict: not what is read here, so nothing waits for them), then the
-// products of `now`.
-template <class S>
-__device__ __forceinline__ void tile_step(char *__restrict__ next, const char *__restrict__ now, bool more,
-                                          const uint8_t *const (&src)[S::kLoadsX + S::kLoadsW], int wave, int x_at, int w_at,
-                                          const float (&s)[S::TT], float4v (&acc)[S::CT][S::TT]) {
-  if (more) {
-#pragma unroll
-    for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i)
-      load_to_lds(src[i], next + (i * S::kWaves + wave) * 1024);
-  }
-  int8v x[S::TT];
-#pragma unroll
-  for (int t = 0; t < S::TT; ++t) {
-    const char *q = now + x_at + t * 16 * kScaleBlock;
-    x[t] = join(*reinterpret_cast<const int4v *>(q), *reinterpret_cast<const int4v *>(now + (x_at ^ 16) + t * 16 * kScaleBlock));
-  }
-#pragma unroll
-  for (int c = 0; c < S::CT; ++c) {
-    const int8v w = join(*reinterpret_cast<const int4v *>(now + w_at + c * 16 * kScaleBlock),
-                         *reinterpret_cast<const int4v *>(now + (w_at ^ 16) + c * 16 * kScaleBlock));
-    float4v part[S::TT];
-#pragma unroll
-    for (int t = 0; t < S::TT; ++t) part[t] = mfma8(w, x[t]);
-#pragma unroll
-    for (int t = 0; t < S::TT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[c][t][i] = fmaf(part[t][i], s[t], acc[c][t][i]);
-  }
+__device__ __forceinline__ void load4_to_lds(const void *src, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(src));
 }
 
 template <int BM, int BN, int WM, int WN, int kOut>
@@ -156,10 +140,11 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
     const int j = tile.row0 + (r < rows ? r : rows - 1);
     return static_cast<size_t>(p.a_rows ? p.a_rows[j] : j);
   };
+  auto block_of = [&](int n) { return n / kScaleBlock < NB ? n / kScaleBlock : NB - 1; };
 
   // sources of this lane's loads: row i * 8 * waves + 8 * wave + lane / 8 of the stage, chunk (lane % 8) ^ (row % 8)
   const int chunk = (lane & 7) ^ (lane >> 3);
-  const uint8_t *src[S::kLoadsX + S::kLoadsW];
+  const uint8_t *src[S::kLoads];
 #pragma unroll
   for (int i = 0; i < S::kLoadsX; ++i)
     src[i] = p.a + a_row((i * S::kWaves + wave) * 8 + (lane >> 3)) * p.K + chunk * 16;
@@ -169,60 +154,116 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
     const int n = n0 + (i * S::kWaves + wave) * 8 + (lane >> 3);
     src[S::kLoadsX + i] = w_e + static_cast<size_t>(n < p.N ? n : p.N - 1) * p.K + chunk * 16;
   }
-  const float *sa[S::TT];
-#pragma unroll
-  for (int t = 0; t < S::TT; ++t) sa[t] = p.a_scale + a_row(wm * (BM / WM) + t * 16 + r16) * KB;
-  int nb = (n0 + wn * (BN / WN)) / kScaleBlock;       // a wavefront's columns share it
-  nb = nb < NB ? nb : NB - 1;
-  const float *sb = p.b_scale + (static_cast<size_t>(tile.e) * NB + nb) * KB;
+  const bool scales_of_rows = wave < BM / 64, scales_of_columns = wave == BM / 64;       // lane i: of column 128 i
+  const float *scale_src = scales_of_rows ? p.a_scale + a_row(wave * 64 + lane) * KB
+                                          : p.b_scale + (static_cast<size_t>(tile.e) * NB + block_of(n0 + lane * kScaleBlock)) * KB;
+  const int nb = block_of(n0 + wn * (BN / WN));      // a wavefront's columns share it
 
-  auto next_sources = [&](int kb) {                   // sources of step kb, from those of kb - 1
-#pragma unroll
-    for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i) src[i] += kScaleBlock;
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)s_tile));
+  auto load_step = [&](int kb, int place) {          // all loads of step kb; the steps come in order
     if (tail && kb == KB - 1 && chunk * 16 >= tail) {
 #pragma unroll
-      for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i) src[i] = reinterpret_cast<const uint8_t *>(&kZeros16);
+      for (int i = 0; i < S::kLoads; ++i) src[i] = reinterpret_cast<const uint8_t *>(&kZeros16);
     }
-  };
-  auto scales = [&](int kb, float (&s)[S::TT]) {
-    const float b = sb[kb];
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds + place * S::kStage + wave * 1024);
 #pragma unroll
-    for (int t = 0; t < S::TT; ++t) s[t] = sa[t][kb] * b;
+    for (int i = 0; i < S::kLoads; ++i) {
+      load16_to_lds(src[i], at + i * S::kWaves * 1024);
+      src[i] += kScaleBlock;
+    }
+    if (scales_of_rows || scales_of_columns)         // the wavefronts' 64 scales each, one behind the other
+      load4_to_lds(scale_src, __builtin_amdgcn_readfirstlane(lds + place * S::kStage + S::kRowsBytes + wave * 256));
+    ++scale_src;
   };
 
-  float4v acc[S::CT][S::TT];
+  const int x_at = (wm * (BM / WM) + r16) * kScaleBlock + ((2 * g) ^ (r16 & 7)) * 16;
+  const int w_at = (BM + wn * (BN / WN) + r16) * kScaleBlock + ((2 * g) ^ (r16 & 7)) * 16;
+  const int sa_at = S::kRowsBytes + 4 * (wm * (BM / WM) + r16), sb_at = S::kRowsBytes + 4 * (BM + wn * (BN / WN) / kScaleBlock);
+  auto fragment = [&](const char *place, int at, int i) {
+    return join(*reinterpret_cast<const int4v *>(place + at + i * 16 * kScaleBlock),
+                *reinterpret_cast<const int4v *>(place + (at ^ 16) + i * 16 * kScaleBlock));
+  };
+  float4v acc[S::CT][S::TT], part[2][S::TT];
+  int8v x[S::TT], w[2];
+  float sa[S::TT], sb, s[S::TT] = {};                // scales as read for the coming step; of the step whose results are scaled
 #pragma unroll
   for (int c = 0; c < S::CT; ++c)
 #pragma unroll
     for (int t = 0; t < S::TT; ++t) acc[c][t] = float4v{0, 0, 0, 0};
-  const int x_at = (wm * (BM / WM) + r16) * kScaleBlock + ((2 * g) ^ (r16 & 7)) * 16;
-  const int w_at = (BM + wn * (BN / WN) + r16) * kScaleBlock + ((2 * g) ^ (r16 & 7)) * 16;
+#pragma unroll
+  for (int t = 0; t < S::TT; ++t) part[(S::CT - 1) & 1][t] = float4v{0, 0, 0, 0};
 
-  if (KB == 1 && tail && chunk * 16 >= tail) {
+  load_step(0, 0);
+  __builtin_amdgcn_s_waitcnt(0x0f70);                // vmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (KB > 1) load_step(1, 1);
+  sb = *reinterpret_cast<const float *>(s_tile + sb_at);
 #pragma unroll
-    for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i) src[i] = reinterpret_cast<const uint8_t *>(&kZeros16);
+  for (int t = 0; t < S::TT; ++t) {
+    x[t] = fragment(s_tile, x_at, t);
+    sa[t] = *reinterpret_cast<const float *>(s_tile + sa_at + 64 * t);
   }
+  w[0] = fragment(s_tile, w_at, 0);
+
+  auto scaled = [&](int c, int t) {
 #pragma unroll
-  for (int i = 0; i < S::kLoadsX + S::kLoadsW; ++i) load_to_lds(src[i], s_tile + (i * S::kWaves + wave) * 1024);
-  float s[S::TT], s_next[S::TT];
-  scales(0, s);
+    for (int i = 0; i < 4; ++i) acc[c][t][i] = fmaf(part[c & 1][t][i], s[t], acc[c][t][i]);
+  };
+  // the sums of columns c exist here: without that the compiler puts all scalings of a step off behind its branch, and
+  // keeps their inputs in registers that there are not
+  auto settled = [&](int c) {
+#pragma unroll
+    for (int t = 0; t < S::TT; ++t) asm volatile("" : "+v"(acc[c][t]));
+  };
   int place = 0;
-  for (int kb = 0; kb < KB; ++kb) {
-    // this step's loads have landed and every wavefront is done with the place that the next step's go to
-    __builtin_amdgcn_s_waitcnt(0x0f70);               // vmcnt(0)
+  for (int kb = 0; kb < KB; ++kb, place ^= 1) {
+    const char *now = s_tile + place * S::kStage;
+    // columns c's products are issued between the scalings of columns c - 1's (of the step before: its last ones)
+#pragma unroll
+    for (int c = 0; c + 1 < S::CT; ++c) {
+      w[(c + 1) & 1] = fragment(now, w_at, c + 1);
+#pragma unroll
+      for (int t = 0; t < S::TT; ++t) {
+        part[c & 1][t] = mfma8(w[c & 1], x[t]);
+        scaled(c ? c - 1 : S::CT - 1, t);
+      }
+      if (c == 0) {
+#pragma unroll
+        for (int t = 0; t < S::TT; ++t) s[t] = sa[t] * sb;
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int t = 0; t < S::TT; ++t) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+      settled(c ? c - 1 : S::CT - 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // the next step's loads have landed, this one's place is read
+    __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const bool more = kb + 1 < KB;
-    if (more) {
-      next_sources(kb + 1);
-      scales(kb + 1, s_next);
-    }
-    tile_step<S>(s_tile + (place ^ 1) * S::kStage, s_tile + place * S::kStage, more, src, wave, x_at, w_at, s, acc);
-    place ^= 1;
+    if (kb + 2 < KB) load_step(kb + 2, place);
+    const char *ahead = s_tile + (place ^ 1) * S::kStage;            // behind the last step: read for nothing
+    constexpr int last = S::CT - 1;
 #pragma unroll
-    for (int t = 0; t < S::TT; ++t) s[t] = s_next[t];
+    for (int t = 0; t < S::TT; ++t) {
+      part[last & 1][t] = mfma8(w[last & 1], x[t]);
+      scaled(last - 1, t);
+      x[t] = fragment(ahead, x_at, t);
+      sa[t] = *reinterpret_cast<const float *>(ahead + sa_at + 64 * t);
+    }
+    w[0] = fragment(ahead, w_at, 0);
+    sb = *reinterpret_cast<const float *>(ahead + sb_at);
+    settled(last - 1);
+    __builtin_amdgcn_sched_barrier(0);
   }
+#pragma unroll
+  for (int t = 0; t < S::TT; ++t) scaled(S::CT - 1, t);
 
   // a lane holds one row and, in every product, four consecutive columns
   const Out *bias = p.bias ? static_cast<const Out *>(p.bias) + static_cast<size_t>(tile.e) * p.N : nullptr;
@@ -472,10 +513,11 @@ int gemm8_out(const Gemm8Args &p, hipStream_t st, const char *what) {
   const int rows = (p.max_rows + owners - 1) / owners;         // of an expert, loads being even
   // (the 8-bit output wants all 128 columns of a scale in one workgroup)
   constexpr int CS = kOut == kGemm8Gelu8 ? 2 : 1;
+  if (g_fp8_form == 2) return launch_tiles<256, 256, 4, 2, kOut>(p, st, what);
   if (rows <= 16) return launch_split<1, 4, CS, kOut>(p, st, what);
   if (rows <= 32) return launch_split<2, 4, CS, kOut>(p, st, what);
   const long long large = static_cast<long long>(p.max_rows / 256 + owners) * ((p.N + 255) / 256);
-  if (rows <= 128 || large < 256) return launch_split<4, 4, 2, kOut>(p, st, what);
+  if (g_fp8_form == 1 || rows <= 128 || large < 256) return launch_split<4, 4, 2, kOut>(p, st, what);
   return launch_tiles<256, 256, 4, 2, kOut>(p, st, what);
 }
 

@@ -15,6 +15,15 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
+@pytest.fixture(params=[0, 1, 2], ids=["by_rule", "k_over_wavefronts", "tiles"], autouse=True)
+def form(request):
+    """Every test in the form that the library picks, and in either of the two."""
+    from ccfuser_amd import ops
+    ops.set_option("fp8_form", request.param)
+    yield request.param
+    ops.set_option("fp8_form", 0)
+
+
 def _randn(seed, *shape, std=1.0):
     return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).cuda()
 
