@@ -5,8 +5,8 @@
 // v_mfma_f32_16x16x128_f8f6f4 contracts one block: its result, from zero, is scaled by a row's and a weight block's scale
 // and added to the sum in fp32, four fused multiply-adds for an instruction of 32 cycles.  Weights are the A operand, so a
 // lane holds four consecutive columns of one row: one scale per lane and 16 rows, and stores of four columns.  (The
-// instruction's own scales are powers of two per 32 elements; weights come with scales of any value.)  The order of K
-// inside a lane's 32 bytes is that of memory for both operands, which is all that a product needs.
+// instruction's own scales are powers of two per 32 elements; weights come with scales of any value.)  A lane's 32
+// bytes are the same ones of either operand, in whatever order of K: all that a product needs.
 //
 // Two kernels.  gemm8_tile_kernel: tiles through LDS, for many rows: bound by the matrix cores.  gemm8_split_kernel: a
 // workgroup's wavefronts cut K among them and read straight from memory, for few rows or few tiles: bound by the weights'
@@ -94,8 +94,9 @@ __device__ __forceinline__ Tile find_tile(const Gemm8Args &p, int pid, int grid,
 // ------------------------------------------------------------------ tiles through LDS
 //
 // BM rows x BN columns, WM x WN wavefronts; a K step is a block of 128, staged by direct loads into one of two LDS places
-// while the other is multiplied.  16-byte chunks of a row lie at chunk ^ (row % 8), which the loads' global addresses
-// apply: eight lanes that read one chunk of eight rows take different banks.  The scales of a step come the same way, a
+// while the other is multiplied.  16-byte chunks of a row lie at chunk ^ (row % 8), which the loads' global addresses apply,
+// and a lane's two chunks are g and g + 4 (g = lane / 16): a read then takes 5 cycles of a wavefront (256 bytes each),
+// with 2 g and 2 g + 1 9, unswizzled 17.  The scales of a step come the same way, a
 // lane per row, and lie by row.
 //
 // A wavefront reads its rows' fragments once a step and its columns' one by one, two in turn.  The step's one barrier stands
@@ -160,28 +161,37 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
   const int nb = block_of(n0 + wn * (BN / WN));      // a wavefront's columns share it
 
   const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)s_tile));
-  auto load_step = [&](int kb, int place) {          // all loads of step kb; the steps come in order
-    if (tail && kb == KB - 1 && chunk * 16 >= tail) {
+  // the loads of step kb in four parts (a wavefront that issues all at once waits for the queue and its products with it);
+  // the steps come in order
+  constexpr int kParts = 4;
+  auto load_part = [&](int kb, int place, int part) {
+    if (part == 0 && tail && kb == KB - 1 && chunk * 16 >= tail) {
 #pragma unroll
       for (int i = 0; i < S::kLoads; ++i) src[i] = reinterpret_cast<const uint8_t *>(&kZeros16);
     }
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds + place * S::kStage + wave * 1024);
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
+    for (int i = part * S::kLoads / kParts; i < (part + 1) * S::kLoads / kParts; ++i) {
       load16_to_lds(src[i], at + i * S::kWaves * 1024);
       src[i] += kScaleBlock;
     }
-    if (scales_of_rows || scales_of_columns)         // the wavefronts' 64 scales each, one behind the other
-      load4_to_lds(scale_src, __builtin_amdgcn_readfirstlane(lds + place * S::kStage + S::kRowsBytes + wave * 256));
-    ++scale_src;
+    if (part == 0) {
+      if (scales_of_rows || scales_of_columns)       // the wavefronts' 64 scales each, one behind the other
+        load4_to_lds(scale_src, __builtin_amdgcn_readfirstlane(lds + place * S::kStage + S::kRowsBytes + wave * 256));
+      ++scale_src;
+    }
+  };
+  auto load_step = [&](int kb, int place) {
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) load_part(kb, place, part);
   };
 
-  const int x_at = (wm * (BM / WM) + r16) * kScaleBlock + ((2 * g) ^ (r16 & 7)) * 16;
-  const int w_at = (BM + wn * (BN / WN) + r16) * kScaleBlock + ((2 * g) ^ (r16 & 7)) * 16;
+  const int x_at = (wm * (BM / WM) + r16) * kScaleBlock + (g ^ (r16 & 7)) * 16;
+  const int w_at = (BM + wn * (BN / WN) + r16) * kScaleBlock + (g ^ (r16 & 7)) * 16;
   const int sa_at = S::kRowsBytes + 4 * (wm * (BM / WM) + r16), sb_at = S::kRowsBytes + 4 * (BM + wn * (BN / WN) / kScaleBlock);
   auto fragment = [&](const char *place, int at, int i) {
     return join(*reinterpret_cast<const int4v *>(place + at + i * 16 * kScaleBlock),
-                *reinterpret_cast<const int4v *>(place + (at ^ 16) + i * 16 * kScaleBlock));
+                *reinterpret_cast<const int4v *>(place + (at ^ 64) + i * 16 * kScaleBlock));
   };
   float4v acc[S::CT][S::TT], part[2][S::TT];
   int8v x[S::TT], w[2];
@@ -198,7 +208,7 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  if (KB > 1) load_step(1, 1);
+  if (KB > 1) load_part(1, 1, 0);
   sb = *reinterpret_cast<const float *>(s_tile + sb_at);
 #pragma unroll
   for (int t = 0; t < S::TT; ++t) {
@@ -241,13 +251,14 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
       }
       settled(c ? c - 1 : S::CT - 1);
       __builtin_amdgcn_sched_barrier(0);
+      if (c < kParts - 1 && kb + 1 < KB) load_part(kb + 1, place ^ 1, c + 1);
     }
     // the next step's loads have landed, this one's place is read
     __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (kb + 2 < KB) load_step(kb + 2, place);
+    if (kb + 2 < KB) load_part(kb + 2, place, 0);
     const char *ahead = s_tile + (place ^ 1) * S::kStage;            // behind the last step: read for nothing
     constexpr int last = S::CT - 1;
 #pragma unroll
