@@ -15,6 +15,7 @@
 #include "gelu.h"
 
 #include <type_traits>
+#include <utility>
 
 namespace ccf {
 int g_fp8_form = 0;          // 0: by the rule of gemm8_out; 1: K cut over the wavefronts always; 2: tiles through LDS always
@@ -27,6 +28,12 @@ __device__ __forceinline__ float4v mfma8(int8v a, int8v b) {
 }
 
 __device__ __forceinline__ int8v join(int4v lo, int4v hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// f(0), f(1), ... f(N - 1), each index a constant
+template <int... I, class F>
+__device__ __forceinline__ void in_turn(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
 
 struct Tile {
   int e, row0, rows, m, n;   // expert (-1: none), first sorted row, rows of the expert from it on, tile indices
@@ -124,91 +131,197 @@ __device__ __forceinline__ void load4_to_lds(const void *src, uint32_t at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(src));
 }
 
+// The experts' tiles in LDS, for a workgroup that runs several: first[e] tiles of rows in front of expert e's, first row of it.
+template <int BM>
+struct TileMap {
+  const int *first, *row;    // [E + 1] each
+  int E, n_tiles;
+
+  // all threads; the caller's barrier follows
+  __device__ __forceinline__ static void build(const Gemm8Args &p, int *first, int *row) {
+    if (threadIdx.x >= 64) return;
+    const int lane = threadIdx.x;
+    int before = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 64) {
+      int lo = 0, hi = 0;
+      if (e0 + lane < p.E) {
+        lo = p.offsets ? p.offsets[e0 + lane] : 0;
+        hi = p.offsets ? p.offsets[e0 + lane + 1] : p.max_rows;
+        lo = lo < p.max_rows ? lo : p.max_rows;
+        hi = hi < p.max_rows ? hi : p.max_rows;
+      }
+      int upto = hi > lo ? (hi - lo + BM - 1) / BM : 0;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(upto, o);
+        upto += lane >= o ? v : 0;
+      }
+      if (e0 + lane < p.E) {
+        if (e0 + lane == 0) first[0] = 0, row[0] = lo;
+        first[e0 + lane + 1] = before + upto;
+        row[e0 + lane + 1] = hi;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+
+  __device__ __forceinline__ int total() const { return __builtin_amdgcn_readfirstlane(first[E]) * n_tiles; }
+
+  // tile t of total(): inside an expert in groups of 8 tiles of rows, columns outside, so that neighbours share both operands
+  __device__ __forceinline__ Tile find(int t) const {
+    const int lane = threadIdx.x & 63;
+    int e0 = 0;
+    unsigned long long past = 0;
+    for (; e0 < E; e0 += 64) {
+      past = __ballot(e0 + lane < E && first[e0 + lane + 1] * n_tiles > t);
+      if (past) break;
+    }
+    const int e = e0 + __ffsll(past) - 1;
+    const int f = __builtin_amdgcn_readfirstlane(first[e]), mts = __builtin_amdgcn_readfirstlane(first[e + 1]) - f;
+    t -= f * n_tiles;
+    const int group = t / (8 * n_tiles), in = t - group * 8 * n_tiles;
+    const int gm = mts - group * 8 < 8 ? mts - group * 8 : 8;
+    Tile r;
+    r.e = e;
+    r.n = in / gm;
+    r.m = group * 8 + in - r.n * gm;
+    r.row0 = __builtin_amdgcn_readfirstlane(row[e]) + r.m * BM;
+    r.rows = __builtin_amdgcn_readfirstlane(row[e + 1]) - r.row0;
+    return r;
+  }
+};
+
+// out[j], j the source's 16 lanes: afterwards the 16 lanes `g` of all four hold what was in[g] of the lanes 16 j ...
+__device__ __forceinline__ void transpose_rows_of_16(uint32_t (&v)[4]) {
+  typedef unsigned uint2v __attribute__((ext_vector_type(2)));
+  uint2v a = __builtin_amdgcn_permlane16_swap(v[0], v[1], false, false), b = __builtin_amdgcn_permlane16_swap(v[2], v[3], false, false);
+  uint2v c = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false), d = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
+  v[0] = c.x;
+  v[1] = d.x;
+  v[2] = c.y;
+  v[3] = d.y;
+}
+
+// Where a lane's loads of a tile's first step start: row i * 8 * waves + 8 * wave + lane / 8 of the stage, in units of 16
+// bytes from p.a or p.b; the scales of row 64 wave + lane, or of column 128 lane, in floats.  (A function, and its caller's
+// advance not another: as closures they kept their captures in memory.)
+template <class S, int BM, int BN>
+__device__ __forceinline__ void tile_sources(const Gemm8Args &p, const Tile &tile, int wave, int lane, int chunk, int KB, int NB,
+                                             uint32_t (&src)[S::kLoads], uint32_t &scale_src) {
+  asm("" : "+v"(lane));                              // what follows from it is made here, not kept over the steps
+  const int rows = tile.rows < BM ? tile.rows : BM, n0 = tile.n * BN;
+  const uint32_t chunks = p.K / 16;
+  auto a_row = [&](int r) {                          // past the end: the last row again, never stored
+    const int j = tile.row0 + (r < rows ? r : rows - 1);
+    return static_cast<uint32_t>(p.a_rows ? p.a_rows[j] : j);
+  };
+#pragma unroll
+  for (int i = 0; i < S::kLoadsX; ++i) src[i] = a_row((i * S::kWaves + wave) * 8 + (lane >> 3)) * chunks + chunk;
+#pragma unroll
+  for (int i = 0; i < S::kLoadsW; ++i) {
+    const int n = n0 + (i * S::kWaves + wave) * 8 + (lane >> 3);
+    src[S::kLoadsX + i] = static_cast<uint32_t>(tile.e * p.N + (n < p.N ? n : p.N - 1)) * chunks + chunk;
+  }
+  if (wave < BM / 64) {
+    scale_src = a_row(wave * 64 + lane) * KB;
+  } else {
+    const int nb = (n0 + lane * kScaleBlock) / kScaleBlock;
+    scale_src = static_cast<uint32_t>(tile.e * NB + (nb < NB ? nb : NB - 1)) * KB;
+  }
+}
+
+// Persistent: a workgroup per CU runs tiles one behind the other, and the steps of all of them are one stream: the next
+// tile's first loads are on their way while this one's last products and its epilogue run.
 template <int BM, int BN, int WM, int WN, int kOut>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
   using S = TileShape<BM, BN, WM, WN>;
   using Out = std::conditional_t<kOut == kGemm8Bf16, bf16_t, half_t>;
-  extern __shared__ __attribute__((aligned(1024))) char s_tile[];
-  const Tile tile = find_tile<BM>(p, blockIdx.x, gridDim.x, n_tiles);
-  if (tile.e < 0) return;
+  extern __shared__ __attribute__((aligned(1024))) char s_tile[];          // two places, then the tile map
+  int *s_map = reinterpret_cast<int *>(s_tile + 2 * S::kStage);
+  TileMap<BM>::build(p, s_map, s_map + p.E + 1);
+  __syncthreads();
+  const TileMap<BM> map{s_map, s_map + p.E + 1, p.E, n_tiles};
+  // workgroup ids go round the 8 XCDs: each XCD takes a run of tiles, which share operands in its L2
+  const int total = map.total(), per = (total + 7) / 8, slots = gridDim.x / 8;
+  const int end = ((blockIdx.x & 7) + 1) * per < total ? ((blockIdx.x & 7) + 1) * per : total;
+  int t_next = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (t_next >= end) return;
+
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int wm = wave / WN, wn = wave % WN;
   const int KB = scale_blocks(p.K), NB = scale_blocks(p.N), tail = p.K % kScaleBlock;
-  const int rows = tile.rows < BM ? tile.rows : BM, n0 = tile.n * BN;
-  auto a_row = [&](int r) {                          // past the end: the last row again, never stored
-    const int j = tile.row0 + (r < rows ? r : rows - 1);
-    return static_cast<size_t>(p.a_rows ? p.a_rows[j] : j);
-  };
-  auto block_of = [&](int n) { return n / kScaleBlock < NB ? n / kScaleBlock : NB - 1; };
+  auto block_of = [&](int n) __attribute__((always_inline)) { return n / kScaleBlock < NB ? n / kScaleBlock : NB - 1; };
 
-  // sources of this lane's loads: row i * 8 * waves + 8 * wave + lane / 8 of the stage, chunk (lane % 8) ^ (row % 8)
-  const int chunk = (lane & 7) ^ (lane >> 3);
-  const uint8_t *src[S::kLoads];
-#pragma unroll
-  for (int i = 0; i < S::kLoadsX; ++i)
-    src[i] = p.a + a_row((i * S::kWaves + wave) * 8 + (lane >> 3)) * p.K + chunk * 16;
-  const uint8_t *w_e = p.b + static_cast<size_t>(tile.e) * p.N * p.K;
-#pragma unroll
-  for (int i = 0; i < S::kLoadsW; ++i) {
-    const int n = n0 + (i * S::kWaves + wave) * 8 + (lane >> 3);
-    src[S::kLoadsX + i] = w_e + static_cast<size_t>(n < p.N ? n : p.N - 1) * p.K + chunk * 16;
-  }
+  const int chunk = (lane & 7) ^ (lane >> 3);        // of a row, that this lane's loads take to place lane % 8
+  uint32_t src[S::kLoads], scale_src;
   const bool scales_of_rows = wave < BM / 64, scales_of_columns = wave == BM / 64;       // lane i: of column 128 i
-  const float *scale_src = scales_of_rows ? p.a_scale + a_row(wave * 64 + lane) * KB
-                                          : p.b_scale + (static_cast<size_t>(tile.e) * NB + block_of(n0 + lane * kScaleBlock)) * KB;
-  const int nb = block_of(n0 + wn * (BN / WN));      // a wavefront's columns share it
-
+  const float *scale_base = p.b_scale;
+  if (scales_of_rows) scale_base = p.a_scale;
+  // the step whose loads are issued next: tile `next` (e < 0: there is none), block next_kb
+  Tile next = map.find(t_next);
+  int next_kb = 0;
+  tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
   const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)s_tile));
-  // the loads of step kb in four parts (a wavefront that issues all at once waits for the queue and its products with it);
-  // the steps come in order
+  // its loads in four parts (a wavefront that issues all at once waits for the queue and its products with it)
   constexpr int kParts = 4;
-  auto load_part = [&](int kb, int place, int part) {
-    if (part == 0 && tail && kb == KB - 1 && chunk * 16 >= tail) {
-#pragma unroll
-      for (int i = 0; i < S::kLoads; ++i) src[i] = reinterpret_cast<const uint8_t *>(&kZeros16);
-    }
+  constexpr std::integral_constant<int, 0> kFirst{};
+  auto load_part = [&](int place, auto PART) __attribute__((always_inline)) {
+    constexpr int part = decltype(PART)::value;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds + place * S::kStage + wave * 1024);
+    const uint8_t *a = p.a + next_kb * kScaleBlock, *b = p.b + next_kb * kScaleBlock;
+    const bool behind = tail && next_kb == KB - 1 && chunk * 16 >= tail;
 #pragma unroll
     for (int i = part * S::kLoads / kParts; i < (part + 1) * S::kLoads / kParts; ++i) {
-      load16_to_lds(src[i], at + i * S::kWaves * 1024);
-      src[i] += kScaleBlock;
+      const uint8_t *q = (i < S::kLoadsX ? a : b) + (static_cast<uint64_t>(src[i]) << 4);
+      load16_to_lds(behind ? reinterpret_cast<const uint8_t *>(&kZeros16) : q, at + i * S::kWaves * 1024);
     }
-    if (part == 0) {
-      if (scales_of_rows || scales_of_columns)       // the wavefronts' 64 scales each, one behind the other
-        load4_to_lds(scale_src, __builtin_amdgcn_readfirstlane(lds + place * S::kStage + S::kRowsBytes + wave * 256));
-      ++scale_src;
-    }
-  };
-  auto load_step = [&](int kb, int place) {
-#pragma unroll
-    for (int part = 0; part < kParts; ++part) load_part(kb, place, part);
+    if (part == 0 && (scales_of_rows || scales_of_columns))          // the wavefronts' 64 scales each, one behind the other
+      load4_to_lds(scale_base + next_kb + scale_src,
+                   __builtin_amdgcn_readfirstlane(lds + place * S::kStage + S::kRowsBytes + wave * 256));
   };
 
   const int x_at = (wm * (BM / WM) + r16) * kScaleBlock + (g ^ (r16 & 7)) * 16;
   const int w_at = (BM + wn * (BN / WN) + r16) * kScaleBlock + (g ^ (r16 & 7)) * 16;
   const int sa_at = S::kRowsBytes + 4 * (wm * (BM / WM) + r16), sb_at = S::kRowsBytes + 4 * (BM + wn * (BN / WN) / kScaleBlock);
-  auto fragment = [&](const char *place, int at, int i) {
+  auto fragment = [&](const char *place, int at, int i) __attribute__((always_inline)) {
     return join(*reinterpret_cast<const int4v *>(place + at + i * 16 * kScaleBlock),
                 *reinterpret_cast<const int4v *>(place + (at ^ 64) + i * 16 * kScaleBlock));
   };
-  float4v acc[S::CT][S::TT], part[2][S::TT];
+  float4v acc[S::CT][S::TT], part[S::TT];
   int8v x[S::TT], w[2];
-  float sa[S::TT], sb, s[S::TT] = {};                // scales as read for the coming step; of the step whose results are scaled
+  float sa[S::TT], sb, s[S::TT];                     // scales as read for the coming step; of the step whose results are scaled
+  auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int c = 0; c < S::CT; ++c)
+    for (int c = 0; c < S::CT; ++c)
 #pragma unroll
-    for (int t = 0; t < S::TT; ++t) acc[c][t] = float4v{0, 0, 0, 0};
+      for (int t = 0; t < S::TT; ++t) acc[c][t] = float4v{0, 0, 0, 0};
 #pragma unroll
-  for (int t = 0; t < S::TT; ++t) part[(S::CT - 1) & 1][t] = float4v{0, 0, 0, 0};
+    for (int t = 0; t < S::TT; ++t) part[t] = float4v{0, 0, 0, 0}, s[t] = 0.0f;
+  };
+  auto scaled = [&](int c, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[c][t][i] = fmaf(part[t][i], s[t], acc[c][t][i]);
+  };
+  // the sums of columns c exist here: without that the compiler puts all scalings of a step off behind its branch, and
+  // keeps their inputs in registers that there are not
+  auto settled = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < S::TT; ++t) asm volatile("" : "+v"(acc[c][t]));
+  };
+  auto meet = [&]() __attribute__((always_inline)) {                                  // all loads have landed, all LDS reads are done
+    __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
 
-  load_step(0, 0);
-  __builtin_amdgcn_s_waitcnt(0x0f70);                // vmcnt(0)
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  if (KB > 1) load_part(1, 1, 0);
+  Tile tile = next;
+  in_turn(std::make_integer_sequence<int, kParts>{}, [&](auto I) __attribute__((always_inline)) { load_part(0, I); });
+  ++next_kb;                                         // (K has two blocks at least)
+  meet();
+  if (next.e >= 0) load_part(1, kFirst);
   sb = *reinterpret_cast<const float *>(s_tile + sb_at);
 #pragma unroll
   for (int t = 0; t < S::TT; ++t) {
@@ -216,55 +329,59 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
     sa[t] = *reinterpret_cast<const float *>(s_tile + sa_at + 64 * t);
   }
   w[0] = fragment(s_tile, w_at, 0);
+  clear();
 
-  auto scaled = [&](int c, int t) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[c][t][i] = fmaf(part[c & 1][t][i], s[t], acc[c][t][i]);
-  };
-  // the sums of columns c exist here: without that the compiler puts all scalings of a step off behind its branch, and
-  // keeps their inputs in registers that there are not
-  auto settled = [&](int c) {
-#pragma unroll
-    for (int t = 0; t < S::TT; ++t) asm volatile("" : "+v"(acc[c][t]));
-  };
-  int place = 0;
-  for (int kb = 0; kb < KB; ++kb, place ^= 1) {
+  int place = 0, kb = 0;
+  while (true) {
     const char *now = s_tile + place * S::kStage;
-    // columns c's products are issued between the scalings of columns c - 1's (of the step before: its last ones)
-#pragma unroll
-    for (int c = 0; c + 1 < S::CT; ++c) {
+    // a product's result is scaled three products later
+    constexpr int last = S::CT - 1;
+    in_turn(std::make_integer_sequence<int, S::CT - 1>{}, [&](auto C) __attribute__((always_inline)) {
+      constexpr int c = decltype(C)::value, c_before = c ? c - 1 : last;           // (the step before's last columns)
       w[(c + 1) & 1] = fragment(now, w_at, c + 1);
 #pragma unroll
-      for (int t = 0; t < S::TT; ++t) {
-        part[c & 1][t] = mfma8(w[c & 1], x[t]);
-        scaled(c ? c - 1 : S::CT - 1, t);
+      for (int t = 0; t < S::TT - 1; ++t) {
+        part[t] = mfma8(w[c & 1], x[t]);
+        scaled(c_before, t + 1);
       }
-      if (c == 0) {
+      if constexpr (c == 0) {
 #pragma unroll
         for (int t = 0; t < S::TT; ++t) s[t] = sa[t] * sb;
       }
+      part[S::TT - 1] = mfma8(w[c & 1], x[S::TT - 1]);
+      scaled(c, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
       for (int t = 0; t < S::TT; ++t) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
       }
-      settled(c ? c - 1 : S::CT - 1);
+      settled(c_before);
       __builtin_amdgcn_sched_barrier(0);
-      if (c < kParts - 1 && kb + 1 < KB) load_part(kb + 1, place ^ 1, c + 1);
-    }
-    // the next step's loads have landed, this one's place is read
-    __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (kb + 2 < KB) load_part(kb + 2, place, 0);
+      if (next.e >= 0) {
+        if constexpr (c < kParts - 1) load_part(place ^ 1, std::integral_constant<int, c + 1>{});
+        if constexpr (c == kParts - 1) {
+          if (++next_kb == KB) {
+            next_kb = 0;
+            t_next += slots;
+            if (t_next < end) {
+              next = map.find(t_next);
+              tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
+            } else {
+              next.e = -1;
+            }
+          }
+        }
+      }
+    });
+    meet();                                          // the next step's loads have landed, this one's place is read
+    if (next.e >= 0) load_part(place, kFirst);
     const char *ahead = s_tile + (place ^ 1) * S::kStage;            // behind the last step: read for nothing
-    constexpr int last = S::CT - 1;
 #pragma unroll
     for (int t = 0; t < S::TT; ++t) {
-      part[last & 1][t] = mfma8(w[last & 1], x[t]);
-      scaled(last - 1, t);
+      part[t] = mfma8(w[last & 1], x[t]);
+      if (t + 1 < S::TT) scaled(last - 1, t + 1);
+      else scaled(last, 0);
       x[t] = fragment(ahead, x_at, t);
       sa[t] = *reinterpret_cast<const float *>(ahead + sa_at + 64 * t);
     }
@@ -272,56 +389,85 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
     sb = *reinterpret_cast<const float *>(ahead + sb_at);
     settled(last - 1);
     __builtin_amdgcn_sched_barrier(0);
-  }
-#pragma unroll
-  for (int t = 0; t < S::TT; ++t) scaled(S::CT - 1, t);
+    place ^= 1;
+    if (++kb < KB) continue;
 
-  // a lane holds one row and, in every product, four consecutive columns
-  const Out *bias = p.bias ? static_cast<const Out *>(p.bias) + static_cast<size_t>(tile.e) * p.N : nullptr;
-  const int col0 = n0 + wn * (BN / WN) + 4 * g;
+    // the tile's end.  A lane holds one row and, in every product, four consecutive columns; of four products' columns it
+    // stores 16 consecutive ones, which it gets from the lanes that hold the same row
 #pragma unroll
-  for (int t = 0; t < S::TT; ++t) {
-    const int r = wm * (BM / WM) + t * 16 + r16;
-    const bool mine = r < rows;
-    const int j = tile.row0 + (mine ? r : 0);
-    const size_t crow = static_cast<size_t>(p.c_rows && mine ? p.c_rows[j] : j);
-    if constexpr (kOut == kGemm8Gelu8) {
-      float top = 0.0f;
+    for (int t = 1; t < S::TT; ++t) scaled(last, t);
+    const int rows = tile.rows < BM ? tile.rows : BM, n0 = tile.n * BN;
+    const Out *bias = p.bias ? static_cast<const Out *>(p.bias) + static_cast<size_t>(tile.e) * p.N : nullptr;
+    const int col0 = n0 + wn * (BN / WN), nb = block_of(col0);       // a wavefront's columns share a scale
+    typedef Out out4 __attribute__((ext_vector_type(4)));
+    out4 b4[S::CT];
 #pragma unroll
-      for (int c = 0; c < S::CT; ++c) {
-        const int col = col0 + 16 * c;
+    for (int c = 0; c < S::CT; ++c) {
+      const int col = col0 + 16 * c + 4 * g;
+      b4[c] = bias && col < p.N ? *reinterpret_cast<const out4 *>(bias + col) : out4{0, 0, 0, 0};
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float b = bias && col < p.N ? static_cast<float>(bias[col + i]) : 0.0f;
-          const float v = col < p.N ? gelu_erf(acc[c][t][i] + b) : 0.0f;
-          acc[c][t][i] = v;
-          top = fmaxf(top, fabsf(v));
-        }
-      }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      float inverse;
-      const float scale = block_scale(top, &inverse);
-      if (mine && col0 < p.N) {
-        if (g == 0) p.scales[crow * NB + nb] = scale;
+    for (int t = 0; t < S::TT; ++t) {
+      const int r = wm * (BM / WM) + t * 16 + r16;
+      const bool mine = r < rows;
+      const int j = tile.row0 + (mine ? r : 0);
+      const size_t crow = static_cast<size_t>(p.c_rows ? p.c_rows[j] : j);
+      if constexpr (kOut == kGemm8Gelu8) {
+        float top = 0.0f;
 #pragma unroll
         for (int c = 0; c < S::CT; ++c)
-          if (col0 + 16 * c < p.N)
-            *reinterpret_cast<int *>(p.codes + crow * p.N + col0 + 16 * c) =
-                pack_fp8(acc[c][t][0] * inverse, acc[c][t][1] * inverse, acc[c][t][2] * inverse, acc[c][t][3] * inverse);
-      }
-    } else if (mine) {
-      typedef Out out4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-      for (int c = 0; c < S::CT; ++c) {
-        const int col = col0 + 16 * c;
-        if (col >= p.N) continue;
-        out4 o;
+          for (int i = 0; i < 4; ++i) {
+            float v = gelu_erf(acc[c][t][i] + static_cast<float>(b4[c][i]));
+            v = col0 + 16 * c + 4 * g < p.N ? v : 0.0f;
+            acc[c][t][i] = v;
+            top = fmaxf(top, fabsf(v));
+          }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        float inverse;
+        const float scale = block_scale(top, &inverse);
+        if (mine && g == 0 && col0 < p.N) p.scales[crow * NB + nb] = scale;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = static_cast<Out>(acc[c][t][i] + (bias ? static_cast<float>(bias[col + i]) : 0.0f));
-        *reinterpret_cast<out4 *>(static_cast<Out *>(p.c) + crow * p.N + col) = o;
+        for (int q = 0; q < S::CT; q += 4) {
+          uint32_t v[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            v[c] = static_cast<uint32_t>(pack_fp8(acc[q + c][t][0] * inverse, acc[q + c][t][1] * inverse,
+                                                  acc[q + c][t][2] * inverse, acc[q + c][t][3] * inverse));
+          transpose_rows_of_16(v);
+          const int col = col0 + 16 * (q + g);
+          uint8_t *at = p.codes + crow * p.N + col;          // 8-byte aligned
+          if (mine && col < p.N) *reinterpret_cast<int2v *>(at) = int2v{static_cast<int>(v[0]), static_cast<int>(v[1])};
+          if (mine && col + 8 < p.N) *reinterpret_cast<int2v *>(at + 8) = int2v{static_cast<int>(v[2]), static_cast<int>(v[3])};
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < S::CT; q += 4) {
+          uint32_t lo[4], hi[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            out4 o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = static_cast<Out>(acc[q + c][t][i] + static_cast<float>(b4[q + c][i]));
+            const int2v words = __builtin_bit_cast(int2v, o);
+            lo[c] = words[0];
+            hi[c] = words[1];
+          }
+          transpose_rows_of_16(lo);
+          transpose_rows_of_16(hi);
+          const int col = col0 + 16 * (q + g);
+          int4v *at = reinterpret_cast<int4v *>(static_cast<Out *>(p.c) + crow * p.N + col);
+          auto word = [](uint32_t v) { return static_cast<int>(v); };
+          if (mine && col < p.N) at[0] = int4v{word(lo[0]), word(hi[0]), word(lo[1]), word(hi[1])};
+          if (mine && col + 8 < p.N) at[1] = int4v{word(lo[2]), word(hi[2]), word(lo[3]), word(hi[3])};
+        }
       }
     }
+    if (next.e < 0) return;
+    tile = next;                                     // whose second step is loaded next (K has two blocks at least)
+    kb = 0;
+    clear();
   }
 }
 
@@ -493,10 +639,12 @@ long long grid_of(const Gemm8Args &p, int bm, int n_tiles) {
 }
 
 template <typename K>
-int launch(K kernel, const Gemm8Args &p, int bm, int bn, int threads, size_t lds, hipStream_t st, const char *what) {
+int launch(K kernel, const Gemm8Args &p, int bm, int bn, int threads, size_t lds, long long most, hipStream_t st,
+           const char *what) {
   const int n_tiles = (p.N + bn - 1) / bn;
-  const long long grid = grid_of(p, bm, n_tiles);
+  long long grid = grid_of(p, bm, n_tiles);
   CCF_REQUIRE(grid < (1ll << 28), CCF_ERR_SHAPE, "%s: too many tiles", what);
+  grid = grid < most ? grid : most;
   if (lds > 65536) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(lds));
@@ -506,16 +654,32 @@ int launch(K kernel, const Gemm8Args &p, int bm, int bn, int threads, size_t lds
   return check_launch(what);
 }
 
+// Compute units of the current device, in whole rounds of the 8 XCDs.
+int compute_units() {
+  static thread_local int cached_dev = -1, cached = 0;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 0;
+  if (dev != cached_dev) {
+    int cus = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
+    cached = cus / 8 * 8;
+    cached_dev = dev;
+  }
+  return cached;
+}
+
 template <int BM, int BN, int WM, int WN, int kOut>
 int launch_tiles(const Gemm8Args &p, hipStream_t st, const char *what) {
   using S = TileShape<BM, BN, WM, WN>;
-  return launch(gemm8_tile_kernel<BM, BN, WM, WN, kOut>, p, BM, BN, S::kThreads, 2 * S::kStage, st, what);
+  const int cus = compute_units();
+  CCF_REQUIRE(cus > 0, CCF_ERR_HIP, "%s: no device", what);
+  return launch(gemm8_tile_kernel<BM, BN, WM, WN, kOut>, p, BM, BN, S::kThreads, 2 * S::kStage + 8 * (p.E + 1), cus, st, what);
 }
 
 template <int TT, int CT, int CS, int kOut>
 int launch_split(const Gemm8Args &p, hipStream_t st, const char *what) {
   using S = SplitShape<TT, CT, CS>;
-  return launch(gemm8_split_kernel<TT, CT, CS, kOut>, p, S::BM, S::BN, 512, S::kLds, st, what);
+  return launch(gemm8_split_kernel<TT, CT, CS, kOut>, p, S::BM, S::BN, 512, S::kLds, 1ll << 28, st, what);
 }
 
 template <int kOut>
@@ -524,11 +688,12 @@ int gemm8_out(const Gemm8Args &p, hipStream_t st, const char *what) {
   const int rows = (p.max_rows + owners - 1) / owners;         // of an expert, loads being even
   // (the 8-bit output wants all 128 columns of a scale in one workgroup)
   constexpr int CS = kOut == kGemm8Gelu8 ? 2 : 1;
-  if (g_fp8_form == 2) return launch_tiles<256, 256, 4, 2, kOut>(p, st, what);
+  const bool can_tile = p.K > kScaleBlock;                     // two steps at least
+  if (g_fp8_form == 2 && can_tile) return launch_tiles<256, 256, 4, 2, kOut>(p, st, what);
   if (rows <= 16) return launch_split<1, 4, CS, kOut>(p, st, what);
   if (rows <= 32) return launch_split<2, 4, CS, kOut>(p, st, what);
   const long long large = static_cast<long long>(p.max_rows / 256 + owners) * ((p.N + 255) / 256);
-  if (g_fp8_form == 1 || rows <= 128 || large < 256) return launch_split<4, 4, 2, kOut>(p, st, what);
+  if (g_fp8_form == 1 || !can_tile || rows <= 128 || large < 256) return launch_split<4, 4, 2, kOut>(p, st, what);
   return launch_tiles<256, 256, 4, 2, kOut>(p, st, what);
 }
 
