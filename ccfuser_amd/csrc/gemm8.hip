@@ -127,6 +127,10 @@ struct TileShape {
 __device__ __forceinline__ void load16_to_lds(const void *src, uint32_t at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src));
 }
+// The same at a 32-bit offset from an address that the wavefront shares.
+__device__ __forceinline__ void load16_to_lds(const void *base, uint32_t offset, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base));
+}
 __device__ __forceinline__ void load4_to_lds(const void *src, uint32_t at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(src));
 }
@@ -202,8 +206,9 @@ __device__ __forceinline__ void transpose_rows_of_16(uint32_t (&v)[4]) {
   v[3] = d.y;
 }
 
-// Where a lane's loads of a tile's first step start: row i * 8 * waves + 8 * wave + lane / 8 of the stage, in units of 16
-// bytes from p.a or p.b; the scales of row 64 wave + lane, or of column 128 lane, in floats.  (A function, and its caller's
+// Where a lane's loads of a tile's first step start, row i * 8 * waves + 8 * wave + lane / 8 of the stage: the tile's rows in
+// units of 16 bytes from p.a, its columns in bytes from the expert's weight; the scales of row 64 wave + lane, or of column
+// 128 lane, in floats.  (A function, and its caller's
 // advance not another: as closures they kept their captures in memory.)
 template <class S, int BM, int BN>
 __device__ __forceinline__ void tile_sources(const Gemm8Args &p, const Tile &tile, int wave, int lane, int chunk, int KB, int NB,
@@ -220,7 +225,7 @@ __device__ __forceinline__ void tile_sources(const Gemm8Args &p, const Tile &til
 #pragma unroll
   for (int i = 0; i < S::kLoadsW; ++i) {
     const int n = n0 + (i * S::kWaves + wave) * 8 + (lane >> 3);
-    src[S::kLoadsX + i] = static_cast<uint32_t>(tile.e * p.N + (n < p.N ? n : p.N - 1)) * chunks + chunk;
+    src[S::kLoadsX + i] = (static_cast<uint32_t>(n < p.N ? n : p.N - 1) * chunks + chunk) * 16;
   }
   if (wave < BM / 64) {
     scale_src = a_row(wave * 64 + lane) * KB;
@@ -270,12 +275,25 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
   auto load_part = [&](int place, auto PART) __attribute__((always_inline)) {
     constexpr int part = decltype(PART)::value;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds + place * S::kStage + wave * 1024);
-    const uint8_t *a = p.a + next_kb * kScaleBlock, *b = p.b + next_kb * kScaleBlock;
-    const bool behind = tail && next_kb == KB - 1 && chunk * 16 >= tail;
+    const uint8_t *a = p.a + next_kb * kScaleBlock;
+    const uint8_t *b = p.b + static_cast<size_t>(next.e) * p.N * p.K + next_kb * kScaleBlock;
+    constexpr int lo = part * S::kLoads / kParts, hi = (part + 1) * S::kLoads / kParts;
+    if (tail && next_kb == KB - 1) {
+      // chunks behind the end of K: zeros for the rows, and for the columns the block's first chunk again (what is no
+      // number there is no number in the sum anyway)
+      const bool behind = chunk * 16 >= tail;
 #pragma unroll
-    for (int i = part * S::kLoads / kParts; i < (part + 1) * S::kLoads / kParts; ++i) {
-      const uint8_t *q = (i < S::kLoadsX ? a : b) + (static_cast<uint64_t>(src[i]) << 4);
-      load16_to_lds(behind ? reinterpret_cast<const uint8_t *>(&kZeros16) : q, at + i * S::kWaves * 1024);
+      for (int i = lo; i < hi; ++i) {
+        const uint8_t *q = a + (static_cast<uint64_t>(src[i]) << 4);
+        if (i < S::kLoadsX) load16_to_lds(behind ? reinterpret_cast<const uint8_t *>(&kZeros16) : q, at + i * S::kWaves * 1024);
+        else load16_to_lds(b, src[i] - (behind ? chunk * 16 : 0), at + i * S::kWaves * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int i = lo; i < hi; ++i) {
+        if (i < S::kLoadsX) load16_to_lds(a + (static_cast<uint64_t>(src[i]) << 4), at + i * S::kWaves * 1024);
+        else load16_to_lds(b, src[i], at + i * S::kWaves * 1024);
+      }
     }
     if (part == 0 && (scales_of_rows || scales_of_columns))          // the wavefronts' 64 scales each, one behind the other
       load4_to_lds(scale_base + next_kb + scale_src,
