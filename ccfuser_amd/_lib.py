@@ -73,6 +73,10 @@ SIGNATURES = {
     "ccf_quantize_weight": (_i, [_p, _i, _i, _i, _i, _p, _p, _p]),
     "ccf_linear_fp8": (_i, [_p, _p, _i, _i, _p, _p, _i, _p, _i, _p, _p]),
     "ccf_ffn1_fp8": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p]),
+    "ccf_moe_few_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "ccf_moe_forward_few": (_i, [_p] * 7 + [_i] * 5 + [_p, _p, _p, _p, _sz, _p]),
+    "ccf_moe_fp8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "ccf_moe_forward_fp8": (_i, [_p] * 11 + [_i] * 6 + [_p, _p, _p, _p, _sz, _p]),
     "ccf_ffn2_fp8": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p]),
 }
 

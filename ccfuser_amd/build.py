@@ -20,7 +20,7 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libccfuser_moe.so"
 PROBE_LIB = HERE / "libccfuser_probe.so"
 SOURCES = ["api.hip", "gate.hip", "route.hip", "rows.hip", "bwd.hip", "few.hip", "thin.hip", "ffn.hip",
-           "norm.hip", "gemm8.hip"]
+           "norm.hip", "gemm8.hip", "few_layer.hip"]
 PROBE_SOURCES = ["probe.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -33,6 +33,7 @@ COMMON = [
 PER_FILE = {
     # the gate's fp32 accumulation order must survive the optimiser
     "gate.hip": ["-ffp-contract=off"],
+    "few_layer.hip": ["-ffp-contract=off"],
     # the 16x16x32 main loop names its accumulation registers itself: nothing of the compiler's may live there
     "ffn.hip": ["-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"],
     "probe.hip": ["-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"],

@@ -10,6 +10,8 @@
 // in place through the row index) and keeps only the activation h and the
 // un-permuted expert output in a caller-owned HBM workspace.
 #include "ccf_common.h"
+#include "few_layer.h"
+#include "gemm8.h"
 #include "plan.h"
 
 namespace ccf {
@@ -121,6 +123,65 @@ BlocksWs carve_blocks(void *ws, int rows, int d, int f, int E) {
   w.ffn_bytes = ccf_ffn_workspace_bytes(rows, E, d, f);
   w.ffn_ws = c.take<char>(w.ffn_bytes);
   w.h = c.take<half_t>(static_cast<size_t>(rows) * f);
+  w.total = c.used;
+  return w;
+}
+
+// The layer for a few tokens: the choice and the activation are all that its second kernel reads of the first.
+struct FewWs {
+  int64_t *idx;        // [n_flat]
+  half_t *score;
+  char *h;             // [n_flat, f] fp16, or codes
+  float *h_scales;
+  size_t total;
+};
+
+FewWs carve_few(void *ws, int tokens, int f, int k, bool fp8) {
+  const size_t n = static_cast<size_t>(tokens) * k;
+  Carver c(ws);
+  FewWs w;
+  w.idx = c.take<int64_t>(n);
+  w.score = c.take<half_t>(n);
+  w.h = c.take<char>(n * f * (fp8 ? 1 : 2));
+  w.h_scales = c.take<float>(fp8 ? n * scale_blocks(f) : 0);
+  w.total = c.used;
+  return w;
+}
+
+struct Moe8Ws {
+  int64_t *idx, *idx_kept;
+  half_t *score;
+  int32_t *counts, *offsets;
+  int64_t *pos;
+  int32_t *src_row, *dst_row, *inv_pos;
+  char *route_ws;
+  size_t route_bytes;
+  uint8_t *x, *h;      // codes [tokens, d], [n_flat, f] and their scales
+  float *x_scales, *h_scales;
+  half_t *y_flat;      // [n_flat, d]
+  size_t total;
+};
+
+Moe8Ws carve_moe8(void *ws, int tokens, int d, int f, int E, int k) {
+  const size_t n = static_cast<size_t>(tokens) * k;
+  Carver c(ws);
+  Moe8Ws w;
+  w.idx = c.take<int64_t>(n);
+  w.idx_kept = c.take<int64_t>(n);
+  w.score = c.take<half_t>(n);
+  w.counts = c.take<int32_t>(E);
+  w.offsets = c.take<int32_t>(E + 1);
+  w.pos = c.take<int64_t>(n);
+  w.src_row = c.take<int32_t>(n);
+  w.dst_row = c.take<int32_t>(n);
+  w.inv_pos = c.take<int32_t>(n);
+  w.route_bytes = ccf_route_workspace_bytes(static_cast<int>(n), E);
+  w.route_ws = c.take<char>(w.route_bytes);
+  w.x = c.take<uint8_t>(static_cast<size_t>(tokens) * d);
+  w.x_scales = c.take<float>(static_cast<size_t>(tokens) * scale_blocks(d));
+  w.h = c.take<uint8_t>(n * f);
+  w.h_scales = c.take<float>(n * scale_blocks(f));
+  w.y_flat = c.take<half_t>(n * d);
   w.total = c.used;
   return w;
 }
@@ -359,4 +420,95 @@ extern "C" int ccf_moe_ffn_blocks(const void *x, int n_tokens, const int64_t *po
     return rc;
   return ffn2_forward(w.h, nullptr, w.flat_rows, w.offsets, rows, num_expert, d_model, d_ffn, w2, b2, nullptr, y,
                       w.ffn_ws, w.ffn_bytes, st, planned2 ? &opt : nullptr, w2_kn != 0);
+}
+
+extern "C" size_t ccf_moe_few_workspace_bytes(int tokens, int d_model, int d_ffn, int num_expert, int top_k) {
+  if (!ccf::few_layer_fits(tokens, d_model, d_ffn, num_expert, top_k)) return 0;
+  return ccf::carve_few(nullptr, tokens, d_ffn, top_k, false).total;
+}
+
+extern "C" int ccf_moe_forward_few(const void *x, const void *wg, const void *bg, const void *w1, const void *b1, const void *w2,
+                                   const void *b2, int tokens, int d_model, int d_ffn, int num_expert, int top_k, void *out,
+                                   int64_t *idx_out, void *score_out, void *workspace, size_t workspace_bytes,
+                                   ccf_stream_t stream) {
+  using namespace ccf;
+  CCF_REQUIRE(tokens >= 0, CCF_ERR_ARG, "moe_forward_few: bad size");
+  if (tokens == 0) return CCF_OK;
+  CCF_REQUIRE(x && wg && w1 && b1 && w2 && b2 && out, CCF_ERR_ARG, "moe_forward_few: null pointer");
+  CCF_REQUIRE(few_layer_fits(tokens, d_model, d_ffn, num_expert, top_k), CCF_ERR_SHAPE,
+              "moe_forward_few: %d tokens of %d / %d, top-%d of %d experts: at most 32 tokens, widths a multiple of 64, "
+              "top_k <= 8 and num_expert <= 1024 are needed", tokens, d_model, d_ffn, top_k, num_expert);
+  CCF_REQUIRE(aligned16(x) && aligned16(wg) && aligned16(w1) && aligned16(w2) && aligned16(out), CCF_ERR_ARG,
+              "moe_forward_few: rows must be 16-byte aligned");
+  const size_t need = ccf_moe_few_workspace_bytes(tokens, d_model, d_ffn, num_expert, top_k);
+  CCF_REQUIRE(workspace && workspace_bytes >= need, CCF_ERR_WORKSPACE, "moe_forward_few: workspace of %zu bytes needed, %zu given",
+              need, workspace_bytes);
+  FewWs w = carve_few(workspace, tokens, d_ffn, top_k, false);
+  auto half = [](const void *p) { return static_cast<const half_t *>(p); };
+  return few_layer(FewLayerArgs{half(x), nullptr, nullptr, half(wg), half(bg), w1, nullptr, half(b1), w2, nullptr, half(b2), tokens,
+                                d_model, d_ffn, num_expert, top_k, idx_out ? idx_out : w.idx,
+                                score_out ? static_cast<half_t *>(score_out) : w.score, w.h, nullptr, static_cast<half_t *>(out)},
+                   false, stream);
+}
+
+extern "C" size_t ccf_moe_fp8_workspace_bytes(int tokens, int d_model, int d_ffn, int num_expert, int top_k) {
+  if (tokens < 0 || d_model <= 0 || d_ffn <= 0 || num_expert <= 0 || top_k <= 0) return 0;
+  if (static_cast<long long>(tokens) * top_k >= (1ll << 31)) return 0;
+  const size_t all = ccf::carve_moe8(nullptr, tokens, d_model, d_ffn, num_expert, top_k).total;
+  const size_t few = ccf::carve_few(nullptr, tokens, d_ffn, top_k, true).total;
+  return all > few ? all : few;
+}
+
+extern "C" int ccf_moe_forward_fp8(const void *x, const void *x_codes, const float *x_scales, const void *wg, const void *bg,
+                                   const void *w1_codes, const float *w1_scales, const void *b1, const void *w2_codes,
+                                   const float *w2_scales, const void *b2, int tokens, int d_model, int d_ffn, int num_expert,
+                                   int top_k, int capacity, void *out, int64_t *idx_out, void *score_out, void *workspace,
+                                   size_t workspace_bytes, ccf_stream_t stream) {
+  using namespace ccf;
+  CCF_REQUIRE(tokens >= 0 && num_expert > 0 && top_k >= 1 && top_k <= 8 && d_model > 0 && d_ffn > 0, CCF_ERR_ARG,
+              "moe_forward_fp8: bad size");
+  CCF_REQUIRE(sizes_ok(static_cast<long long>(tokens) * top_k, d_model, d_ffn) && d_model % 64 == 0 && d_ffn % 64 == 0 &&
+                  num_expert <= 1024 && top_k <= num_expert, CCF_ERR_SHAPE,
+              "moe_forward_fp8: %d tokens of %d / %d, top-%d of %d experts: widths a multiple of 64, top_k <= num_expert <= 1024 "
+              "and tokens * top_k < 2^31 are needed", tokens, d_model, d_ffn, top_k, num_expert);
+  if (tokens == 0) return CCF_OK;
+  CCF_REQUIRE(x && wg && w1_codes && w1_scales && w2_codes && w2_scales && out && !x_codes == !x_scales, CCF_ERR_ARG,
+              "moe_forward_fp8: null pointer");
+  CCF_REQUIRE(aligned16(x) && aligned16(x_codes) && aligned16(wg) && aligned16(w1_codes) && aligned16(w2_codes) && aligned16(out) &&
+                  aligned16(b1) && aligned16(b2), CCF_ERR_ARG, "moe_forward_fp8: rows must be 16-byte aligned");
+  const size_t need = ccf_moe_fp8_workspace_bytes(tokens, d_model, d_ffn, num_expert, top_k);
+  CCF_REQUIRE(workspace && workspace_bytes >= need, CCF_ERR_WORKSPACE, "moe_forward_fp8: workspace of %zu bytes needed, %zu given",
+              need, workspace_bytes);
+  auto half = [](const void *p) { return static_cast<const half_t *>(p); };
+  auto bytes = [](const void *p) { return static_cast<const uint8_t *>(p); };
+  hipStream_t st = as_stream(stream);
+  // no expert can get more rows than there are tokens: a capacity of as many drops nothing
+  if (few_layer_fits(tokens, d_model, d_ffn, num_expert, top_k) && (capacity < 0 || capacity >= tokens)) {
+    FewWs w = carve_few(workspace, tokens, d_ffn, top_k, true);
+    return few_layer(FewLayerArgs{half(x), bytes(x_codes), x_scales, half(wg), half(bg), w1_codes, w1_scales, half(b1), w2_codes,
+                                  w2_scales, half(b2), tokens, d_model, d_ffn, num_expert, top_k, idx_out ? idx_out : w.idx,
+                                  score_out ? static_cast<half_t *>(score_out) : w.score, w.h, w.h_scales, static_cast<half_t *>(out)},
+                     true, stream);
+  }
+  Moe8Ws w = carve_moe8(workspace, tokens, d_model, d_ffn, num_expert, top_k);
+  if (idx_out) w.idx_kept = idx_out;
+  if (score_out) w.score = static_cast<half_t *>(score_out);
+  const int n = tokens * top_k;
+  if (int rc = ccf_gate_route(x, wg, bg, tokens, d_model, num_expert, top_k, CCF_F16, capacity, w.idx, w.score, w.counts, w.offsets,
+                              w.pos, w.src_row, w.dst_row, w.inv_pos, w.idx_kept, w.route_ws, w.route_bytes, stream))
+    return rc;
+  if (!x_codes) {
+    if (int rc = launch_quantize_rows(x, tokens, d_model, CCF_F16, w.x, w.x_scales, st)) return rc;
+    x_codes = w.x;
+    x_scales = w.x_scales;
+  }
+  if (int rc = ccf_ffn1_fp8(x_codes, x_scales, w.src_row, w.offsets, n, num_expert, d_model, d_ffn, w1_codes, w1_scales, b1, w.h,
+                            w.h_scales, stream))
+    return rc;
+  const bool direct = top_k == 1 && capacity < 0;       // a token's one score is 1
+  if (int rc = ccf_ffn2_fp8(w.h, w.h_scales, w.dst_row, w.offsets, n, num_expert, d_model, d_ffn, w2_codes, w2_scales, b2,
+                            direct ? out : w.y_flat, stream))
+    return rc;
+  return direct ? static_cast<int>(CCF_OK) : launch_combine(w.y_flat, w.score, w.inv_pos, static_cast<half_t *>(out), tokens, top_k,
+                                                            d_model, st);
 }

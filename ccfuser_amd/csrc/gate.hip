@@ -23,6 +23,7 @@
 // and add separate (two roundings): both on the vector unit, or with many tokens
 // the multiplies as MFMAs onto zero.
 #include "ccf_common.h"
+#include "gate_select.h"
 #include "mfma_f32.h"
 #include "plan.h"
 
@@ -35,75 +36,7 @@ int g_gate_slots = 0;    // parts of K a wavefront works on at a time (1, 2, 4);
 int g_gate_stream = -1;  // 1: every wavefront takes its tokens through all of K alone; 0: never; -1: with many tokens
 namespace {
 
-constexpr int kMaxTopK = 8;
-constexpr int kPart = 128;          // K elements of a part
 constexpr int kMaxWaves = 8;
-
-template <typename T>
-__device__ inline float round_to(float v) {
-  return static_cast<float>(static_cast<T>(v));
-}
-
-__device__ inline bool better(float v, int id, float bv, int bid) {
-  return v > bv || (v == bv && id < bid);
-}
-
-// The k best of a token so far (k <= KS), best first; ties keep the lower expert id.
-template <int KS>
-struct Best {
-  float v[KS];
-  int id[KS];
-  __device__ inline void clear() {
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      v[s] = -INFINITY;
-      id[s] = INT_MAX;
-    }
-  }
-  __device__ inline void offer(float nv, int nid, int k) {
-    if constexpr (KS > 2) {                        // long lists: most offers end at the last kept entry
-      float lv = v[0];
-      int li = id[0];
-#pragma unroll
-      for (int s = 1; s < KS; ++s)
-        if (s == k - 1) {
-          lv = v[s];
-          li = id[s];
-        }
-      if (!better(nv, nid, lv, li)) return;        // not among the k best
-    }
-    bool beats[KS];                                // short lists: no branch
-#pragma unroll
-    for (int s = 0; s < KS; ++s) beats[s] = better(nv, nid, v[s], id[s]);
-#pragma unroll
-    for (int s = KS - 1; s >= 0; --s) {
-      if (s < k) {
-        const int up = s > 0 ? s - 1 : 0;
-        const bool ahead = s > 0 && beats[up];     // belongs further up: slot s takes its upper neighbour
-        v[s] = ahead ? v[up] : (beats[s] ? nv : v[s]);
-        id[s] = ahead ? id[up] : (beats[s] ? nid : id[s]);
-      }
-    }
-  }
-  // softmax over the k selected logits (slot 0 holds the maximum) and the writes
-  template <typename T>
-  __device__ inline void write(int t, int k, int64_t *__restrict__ idx_out, T *__restrict__ score_out) const {
-    float ex[KS];
-    float sum = 0.0f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      ex[s] = (s < k) ? expf(v[s] - v[0]) : 0.0f;
-      sum += ex[s];
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if (s < k) {
-        idx_out[static_cast<size_t>(t) * k + s] = static_cast<int64_t>(id[s]);
-        score_out[static_cast<size_t>(t) * k + s] = static_cast<T>(ex[s] / sum);
-      }
-    }
-  }
-};
 
 // Leaves how many of the workgroup's token slots chose each expert, for the routing stage: the selection threads hold the
 // ids, so the routing needs no pass of its own over idx to count them.  `row`: E ints of LDS that nothing else uses from

@@ -956,3 +956,83 @@ def ffn2_fp8(h, dst_row: Optional[torch.Tensor], offsets: torch.Tensor, max_rows
         _lib.call("ccf_ffn2_fp8", _ptr(codes), _ptr(scale), _ptr(dst_row), _ptr(offsets), int(max_rows), E, d, f, _ptr(w2_codes),
                   _ptr(w2_scale), _ptr(b2), _ptr(y), _stream(codes))
     return y
+
+
+FEW_TOKENS = 32              # most tokens of ``moe_forward_few``
+
+
+def _check_layer(x, wg, bg, top_k: int, what: str) -> None:
+    if isinstance(x, torch.Tensor) and x.dtype != torch.float16:
+        raise TypeError("moe input data type must be float 16")
+    _check(x, "x", dtype=torch.float16, ndim=2)
+    _check(wg, "gate weight", dtype=torch.float16, ndim=2)
+    if bg is not None:
+        _check(bg, "gate bias", dtype=torch.float16, ndim=1)
+    if wg.shape[1] != x.shape[1] or (bg is not None and bg.shape[0] != wg.shape[0]):
+        raise ValueError(f"{what}: gate weight/bias shapes do not match the input")
+    if not 1 <= top_k <= min(8, wg.shape[0]):
+        raise ValueError(f"{what}: top_k={top_k} outside 1..{min(8, wg.shape[0])}")
+
+
+def moe_forward_few(x: torch.Tensor, wg: torch.Tensor, bg: Optional[torch.Tensor], w1: torch.Tensor, b1: torch.Tensor,
+                    w2: torch.Tensor, b2: torch.Tensor, top_k: int, return_routing: bool = False,
+                    workspace: Optional[torch.Tensor] = None, spare_experts: bool = False):
+    """``moe_forward`` for at most 32 tokens in two kernels: out [T, d] fp16 (and ``idx`` and ``score`` on request).  The
+    choice is the gate's, bit for bit; outputs differ from ``moe_forward``'s in the order of sums and by one rounding.
+    ``spare_experts`` as in ``moe_forward``."""
+    top_k = int(top_k)
+    _check_layer(x, wg, bg, top_k, "moe_forward_few")
+    _check_expert(w1, b1, "ffn1")
+    _check_expert(w2, b2, "ffn2")
+    T, d = x.shape
+    E, (slots, f, d1) = wg.shape[0], w1.shape
+    fits = min(slots, w2.shape[0]) >= E if spare_experts else slots == w2.shape[0] == E
+    if d1 != d or not fits or tuple(w2.shape[1:]) != (d, f):
+        raise ValueError("moe_forward_few: weight shapes do not match")
+    if T > FEW_TOKENS:
+        raise ValueError(f"moe_forward_few takes at most {FEW_TOKENS} tokens, got {T}")
+    _same_device(x, wg, bg, w1, b1, w2, b2, workspace)
+    out = torch.empty_like(x)
+    idx = torch.empty(T, top_k, dtype=torch.int64, device=x.device) if return_routing else None
+    score = torch.empty(T, top_k, dtype=torch.float16, device=x.device) if return_routing else None
+    with _on(x):
+        ws = workspace if workspace is not None else _workspace(
+            _lib.lib().ccf_moe_few_workspace_bytes(T, d, f, E, top_k), x)
+        _lib.call("ccf_moe_forward_few", _ptr(x), _ptr(wg), _ptr(bg), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), T, d, f, E, top_k,
+                  _ptr(out), _ptr(idx), _ptr(score), _ptr(ws), ws.numel(), _stream(x))
+    return (out, {"idx": idx, "score": score}) if return_routing else out
+
+
+def moe_forward_fp8(x: torch.Tensor, wg: torch.Tensor, bg: Optional[torch.Tensor], w1_codes: torch.Tensor,
+                    w1_scale: torch.Tensor, b1: Optional[torch.Tensor], w2_codes: torch.Tensor, w2_scale: torch.Tensor,
+                    b2: Optional[torch.Tensor], top_k: int, capacity: int = -1, x_fp8=None, return_routing: bool = False,
+                    workspace: Optional[torch.Tensor] = None):
+    """``moe_forward`` on experts in 8 bits: out [T, d] fp16 (and ``idx``, after the capacity limit, and ``score`` on request).
+    The gate scores ``x`` in fp16; ``x_fp8``, a pair as ``quantize_rows`` or ``rms_norm`` give it, is what the experts
+    read, quantised by the call without it.  Weights [E, f, d] and [E, d, f] as ``quantize_weight`` returns them, or any
+    codes with any scale per 128 x 128 block.  Few tokens take two kernels, as ``moe_forward_few``.  Not differentiable."""
+    top_k = int(top_k)
+    _check_layer(x, wg, bg, top_k, "moe_forward_fp8")
+    _check_expert_fp8(w1_codes, w1_scale, b1, "ffn1")
+    _check_expert_fp8(w2_codes, w2_scale, b2, "ffn2")
+    T, d = x.shape
+    E, f, d1 = w1_codes.shape
+    if d1 != d or tuple(w2_codes.shape) != (E, d, f) or wg.shape[0] != E:
+        raise ValueError("moe_forward_fp8: weight shapes do not match (one GPU: the gate scores the local experts)")
+    codes = scale = None
+    if x_fp8 is not None:
+        codes, scale = x_fp8
+        _check_fp8(codes, scale, "x_fp8", False, 2)
+        if codes.shape != x.shape:
+            raise ValueError("moe_forward_fp8: x and x_fp8 differ in shape")
+    _same_device(x, wg, bg, w1_codes, w2_codes, codes, workspace)
+    out = torch.empty_like(x)
+    idx = torch.empty(T, top_k, dtype=torch.int64, device=x.device) if return_routing else None
+    score = torch.empty(T, top_k, dtype=torch.float16, device=x.device) if return_routing else None
+    with _on(x):
+        ws = workspace if workspace is not None else _workspace(
+            _lib.lib().ccf_moe_fp8_workspace_bytes(T, d, f, E, top_k), x)
+        _lib.call("ccf_moe_forward_fp8", _ptr(x), _ptr(codes), _ptr(scale), _ptr(wg), _ptr(bg), _ptr(w1_codes), _ptr(w1_scale),
+                  _ptr(b1), _ptr(w2_codes), _ptr(w2_scale), _ptr(b2), T, d, f, E, top_k, int(capacity), _ptr(out), _ptr(idx),
+                  _ptr(score), _ptr(ws), ws.numel(), _stream(x))
+    return (out, {"idx": idx, "score": score}) if return_routing else out

@@ -97,6 +97,8 @@ const char *ccf_last_error(void);
  *                     routing stage's last launch sums itself instead of running a scan launch; in
  *                     ccf_moe_forward the gate kernel leaves such a table when it fits (and top_k is a power
  *                     of two), and the routing stage is then one launch.  0 = always histogram, scan, pos
+ *   "fp8_form"        0 (default): products in 8 bits run as 256-row tiles through LDS or, for few rows or few tiles, with K
+ *                     cut over the wavefronts of a workgroup; 1 = the second always, 2 = the first (K of 256 and more)
  *   "gate_slots"      0, 1, 2 or 4: parts of K a gate wavefront works on at a time, which divides the tokens
  *                     of a workgroup by the same number (0 = chosen by the token count)
  *   "dgrad_transpose" 0/1: the backward's input-gradient GEMM runs on a transposed copy of the
@@ -666,6 +668,37 @@ int ccf_ffn1_fp8(const void *x_codes, const float *x_scales, const int32_t *src_
 int ccf_ffn2_fp8(const void *h_codes, const float *h_scales, const int32_t *dst_row, const int32_t *offsets, int max_rows,
                  int num_expert, int d_model, int d_ffn, const void *w2_codes, const float *w2_scales, const void *b2, void *y,
                  ccf_stream_t stream);
+
+/* Bytes of workspace ccf_moe_forward_few needs; 0: not a size it takes (no counterpart in the reference). */
+size_t ccf_moe_few_workspace_bytes(int tokens, int d_model, int d_ffn, int num_expert, int top_k);
+
+/*
+ * ccf_moe_forward for a few tokens in two kernels: gate, choice, FFN1 and GELU; FFN2 and the combine
+ * (mix_moe/csrc/mix_moe.h:507-598).  The choice and its scores are the gate's, bit for bit; the outputs come of other sums
+ * than ccf_moe_forward's and one rounding less (an expert's output is not rounded to fp16 before the combine).
+ * At most 32 tokens, widths a multiple of 64, no capacity limit (an expert gets as many rows as there are tokens at most).
+ * With more experts, tokens or a wider model than a workgroup gates for itself, the gate is a launch in front.
+ * idx_out int64 [tokens*top_k] (-1: no expert), score_out fp16 [tokens*top_k], NULL to skip.
+ */
+int ccf_moe_forward_few(const void *x, const void *wg, const void *bg, const void *w1, const void *b1, const void *w2,
+                        const void *b2, int tokens, int d_model, int d_ffn, int num_expert, int top_k, void *out,
+                        int64_t *idx_out, void *score_out, void *workspace, size_t workspace_bytes, ccf_stream_t stream);
+
+/* Bytes of workspace ccf_moe_forward_fp8 needs (no counterpart in the reference). */
+size_t ccf_moe_fp8_workspace_bytes(int tokens, int d_model, int d_ffn, int num_expert, int top_k);
+
+/*
+ * ccf_moe_forward on experts in 8 bits: gate in fp16, ccf_ffn1_fp8, ccf_ffn2_fp8, combine; at most 32 tokens in the two
+ * kernels of ccf_moe_forward_few (mix_moe/csrc/mix_moe.h:507-598 in fp16).
+ *   x [tokens, d_model] fp16 is what the gate scores; x_codes and x_scales, the same rows in 8 bits for the experts, may be
+ *   NULL (quantised by the call).  Weights as in ccf_ffn1_fp8 and ccf_ffn2_fp8, b1 and b2 fp16 or NULL; capacity as in
+ *   ccf_route; idx_out (after capacity) and score_out as in ccf_moe_forward.  Widths are multiples of 64.
+ */
+int ccf_moe_forward_fp8(const void *x, const void *x_codes, const float *x_scales, const void *wg, const void *bg,
+                        const void *w1_codes, const float *w1_scales, const void *b1, const void *w2_codes,
+                        const float *w2_scales, const void *b2, int tokens, int d_model, int d_ffn, int num_expert, int top_k,
+                        int capacity, void *out, int64_t *idx_out, void *score_out, void *workspace, size_t workspace_bytes,
+                        ccf_stream_t stream);
 
 #ifdef __cplusplus
 }
