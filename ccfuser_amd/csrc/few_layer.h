@@ -25,6 +25,8 @@ struct FewLayerArgs {
 };
 
 bool few_layer_fits(int tokens, int d, int f, int E, int k);
+// Whether the first kernel quantises the tokens for itself; otherwise the caller brings them in 8 bits.
+bool few_layer_quantises(int tokens, int d);
 int few_layer(const FewLayerArgs &p, bool fp8, ccf_stream_t stream);
 
 }  // namespace ccf

@@ -31,7 +31,7 @@ constexpr int kThreads = 512, kWaves = kThreads / 64;
 
 __device__ const int4v kZeros16 = {0, 0, 0, 0};    // what lanes behind the end of K read
 
-enum { kHalf = 0, kCodes = 1, kQuantise = 2 };     // fp16 weights; e4m3 ones, with rows in 8 bits or quantised here
+enum { kHalf = 0, kCodes = 1, kQuantise = 2 };     // fp16 weights; e4m3 ones, with rows in 8 bits or quantised here into LDS
 
 __device__ __forceinline__ int8v join(int4v lo, int4v hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
 
@@ -92,67 +92,110 @@ struct Slots {
   }
 };
 
-// LDS of the gate: expert rows, token rows, part sums, logits
+// LDS of the gate: a slice of the expert rows (32 elements of every part), token rows, part sums, logits
 struct GateLds {
   int x, part, logit, bytes;
 };
+constexpr int kSliceRow = 80;                      // a part's 64 bytes of a slice + 16: bank spread
+constexpr int kGateChains = 512;                   // most parts of expert rows: their pieces are on their way in registers
 __host__ __device__ inline GateLds gate_lds(int T, int E, int nparts) {
   GateLds l;
-  l.x = E * nparts * 256;
+  l.x = E * nparts * kSliceRow;
   l.part = l.x + T * nparts * 256;
   l.logit = l.part + 4 * T * E * (nparts + 1);
-  l.bytes = l.logit + 4 * T * (E + 1);
+  l.bytes = (l.logit + 4 * T * (E + 1) + 15) / 16 * 16;
   return l;
 }
 
 // The gate's choice for all tokens: chains of fused multiply-adds over parts of 128 elements from zero, the parts' sums in
-// ascending order, the bias last, one rounding to fp16.  Rows lie in LDS in 16-byte pieces, piece c of part i at
-// c ^ (i % 16), so that lanes on neighbouring parts read other banks.
+// ascending order, the bias last, one rounding to fp16.  The expert rows are loaded at once, 16 bytes at a time, into
+// registers and pass through LDS in four slices, so that they leave room for a second workgroup on the CU.  Token rows lie
+// in LDS in 16-byte pieces, piece c of part i at c ^ (i % 16), so that lanes on neighbouring parts read other banks.
 __device__ __forceinline__ void gate_here(const FewLayerArgs &p, char *s_raw, Slots &slots) {
-  const int T = p.tokens, d = p.d, E = p.E, k = p.k, nparts = (d + kPart - 1) / kPart;
+  const int T = p.tokens, d = p.d, E = p.E, k = p.k, nparts = (d + kPart - 1) / kPart, chains = E * nparts;
   const GateLds at = gate_lds(T, E, nparts);
+  const FastDiv by_parts(nparts), by_chains(chains), by_experts(E);
   float *s_part = reinterpret_cast<float *>(s_raw + at.part), *s_logit = reinterpret_cast<float *>(s_raw + at.logit);
-  auto fetch = [&](const half_t *base, int rows, int to) {
-    const int pieces = rows * nparts * 16;
-    for (int s = threadIdx.x; s < pieces; s += kThreads) {
-      const int i = s >> 4, r = i / nparts, part = i - r * nparts, c = s & 15, kk = part * kPart + c * 8;
-      const half8 v = kk < d ? *reinterpret_cast<const half8 *>(base + static_cast<size_t>(r) * d + kk) : half8{0, 0, 0, 0, 0, 0, 0, 0};
-      *reinterpret_cast<half8 *>(s_raw + to + i * 256 + ((c ^ (i & 15)) << 4)) = v;
+  constexpr int kSlices = 4, kPer = kGateChains * 4 / kThreads;            // pieces of a slice to a thread
+  half8 piece_of[kSlices][kPer];
+#pragma unroll
+  for (int s = 0; s < kSlices; ++s)
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int q = i * kThreads + threadIdx.x, chain = q >> 2, e = by_parts.div(chain);
+      const int kk = (chain - e * nparts) * kPart + s * 32 + (q & 3) * 8;
+      piece_of[s][i] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (chain < chains && kk < d) piece_of[s][i] = *reinterpret_cast<const half8 *>(p.wg + static_cast<size_t>(e) * d + kk);
     }
-  };
-  fetch(p.wg, E, 0);
-  fetch(p.x, T, at.x);
-  __syncthreads();
-  const int chains = E * nparts;
-  for (int q = threadIdx.x; q < T * chains; q += kThreads) {
-    const int t = q / chains, chain = q - t * chains, part = chain % nparts, xi = t * nparts + part;
-    const char *wr = s_raw + chain * 256, *xr = s_raw + at.x + xi * 256;
-    const int len = d - part * kPart;
-    float acc = 0.0f;
+  const int x_pieces = T * nparts * 16;
+#pragma unroll 4
+  for (int q = threadIdx.x; q < x_pieces; q += kThreads) {
+    const int i = q >> 4, t = by_parts.div(i), c = q & 15, kk = (i - t * nparts) * kPart + c * 8;
+    half8 v = half8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (kk < d) v = *reinterpret_cast<const half8 *>(p.x + static_cast<size_t>(t) * d + kk);
+    *reinterpret_cast<half8 *>(s_raw + at.x + i * 256 + ((c ^ (i & 15)) << 4)) = v;
+  }
+  // a thread's chains (the caller sees to it that two are enough)
+  constexpr int kChains = 2;
+  float acc[kChains];
+  int chain_of[kChains], x_of[kChains], len_of[kChains];
+  bool live[kChains];
 #pragma unroll
-    for (int c = 0; c < kPart / 8; ++c) {
-      const half8 wv = *reinterpret_cast<const half8 *>(wr + ((c ^ (chain & 15)) << 4));
-      const half8 xv = *reinterpret_cast<const half8 *>(xr + ((c ^ (xi & 15)) << 4));
-      if (c * 8 < len) {
+  for (int j = 0; j < kChains; ++j) {
+    const int q = j * kThreads + threadIdx.x, t = by_chains.div(q);
+    live[j] = q < T * chains;
+    chain_of[j] = q - t * chains;
+    const int part = chain_of[j] - by_parts.div(chain_of[j]) * nparts;
+    x_of[j] = t * nparts + part;
+    len_of[j] = d - part * kPart;
+    acc[j] = 0.0f;
+  }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc = __builtin_fmaf(static_cast<float>(xv[j]), static_cast<float>(wv[j]), acc);
+  for (int s = 0; s < kSlices; ++s) {
+    if (s) __syncthreads();                        // the last slice is read
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int q = i * kThreads + threadIdx.x, chain = q >> 2;
+      if (chain < chains) *reinterpret_cast<half8 *>(s_raw + chain * kSliceRow + (q & 3) * 16) = piece_of[s][i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kChains; ++j) {
+      if (!live[j]) continue;
+      const char *wr = s_raw + chain_of[j] * kSliceRow, *xr = s_raw + at.x + x_of[j] * 256;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const half8 wv = *reinterpret_cast<const half8 *>(wr + c * 16);
+        const half8 xv = *reinterpret_cast<const half8 *>(xr + (((s * 4 + c) ^ (x_of[j] & 15)) << 4));
+        if (s * 32 + c * 8 < len_of[j]) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[j] = __builtin_fmaf(static_cast<float>(xv[i]), static_cast<float>(wv[i]), acc[j]);
+        }
       }
     }
-    s_part[(t * E + chain / nparts) * (nparts + 1) + part] = acc;
   }
+#pragma unroll
+  for (int j = 0; j < kChains; ++j)
+    if (live[j]) {
+      const int row = by_parts.div(x_of[j]) * E + by_parts.div(chain_of[j]);           // token, expert
+      s_part[row * (nparts + 1) + x_of[j] - by_parts.div(x_of[j]) * nparts] = acc[j];
+    }
   __syncthreads();
   for (int i = threadIdx.x; i < T * E; i += kThreads) {
     const float *ps = s_part + i * (nparts + 1);
     float v = ps[0];
+#pragma unroll 8
     for (int q = 1; q < nparts; ++q) v = v + ps[q];
-    if (p.bg) v = v + static_cast<float>(p.bg[i % E]);
-    s_logit[i / E * (E + 1) + i % E] = round_to<half_t>(v);
+    const int t = by_experts.div(i), e = i - t * E;
+    if (p.bg) v = v + static_cast<float>(p.bg[e]);
+    s_logit[t * (E + 1) + e] = round_to<half_t>(v);
   }
   __syncthreads();
   if (static_cast<int>(threadIdx.x) < T) {
     const int t = threadIdx.x;
     Best<kMaxTopK> best;
     best.clear();
+#pragma unroll 8
     for (int e = 0; e < E; ++e) best.offer(s_logit[t * (E + 1) + e], e, k);
     int64_t idx[kMaxTopK];
     half_t score[kMaxTopK];
@@ -169,16 +212,69 @@ __device__ __forceinline__ void gate_here(const FewLayerArgs &p, char *s_raw, Sl
   }
 }
 
+// Tokens in 8 bits in LDS: rows of d codes, 16 bytes apart beyond that (16 rows on as many banks), then their scales.
+struct RowsLds {
+  int ld, scales, bytes;
+};
+__host__ __device__ inline RowsLds rows_lds(int T, int d) {
+  RowsLds l;
+  l.ld = (d + 127) / 128 * 128 + 16;
+  l.scales = T * l.ld;
+  l.bytes = (l.scales + 4 * T * scale_blocks(d) + 15) / 16 * 16;
+  return l;
+}
+
+// As ccf_quantize_rows: 16 lanes to a block of 128.  Codes behind the end of K are zeros.  The caller's barrier follows.
+__device__ __forceinline__ void quantise_here(const FewLayerArgs &p, char *s_rows, const RowsLds &at) {
+  const int blocks = scale_blocks(p.d);
+  const FastDiv by_blocks(blocks);
+  const int pieces = p.tokens * blocks * 16;
+  constexpr int kAhead = 4;                        // loads on their way
+  for (int q0 = threadIdx.x; q0 < pieces; q0 += kAhead * kThreads) {
+    half8 v[kAhead];
+    int row[kAhead], col[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int q = q0 + a * kThreads, i = q >> 4;
+      row[a] = by_blocks.div(i);
+      col[a] = (i - row[a] * blocks) * kScaleBlock + (q & 15) * 8;
+      v[a] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (q < pieces && col[a] < p.d) v[a] = *reinterpret_cast<const half8 *>(p.x + static_cast<size_t>(row[a]) * p.d + col[a]);
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int q = q0 + a * kThreads;
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(static_cast<float>(v[a][j])));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+      float inverse;
+      const float scale = block_scale(top, &inverse);
+      auto four = [&](int j) {
+        return pack_fp8(static_cast<float>(v[a][j]) * inverse, static_cast<float>(v[a][j + 1]) * inverse,
+                        static_cast<float>(v[a][j + 2]) * inverse, static_cast<float>(v[a][j + 3]) * inverse);
+      };
+      if (q >= pieces) continue;
+      *reinterpret_cast<int2v *>(s_rows + row[a] * at.ld + col[a]) = int2v{four(0), four(4)};
+      if ((q & 15) == 0) *reinterpret_cast<float *>(s_rows + at.scales + 4 * (q >> 4)) = scale;
+    }
+  }
+}
+
 // 16 RB tokens; a workgroup's columns: 64 of fp16 weights, whose K all eight wavefronts cut among them, 128 in 8 bits, four
 // wavefronts to either half.
 template <int kIn, int RB>
-__global__ void __launch_bounds__(kThreads, kIn == kHalf && RB == 1 ? 4 : 2)
+__global__ void __launch_bounds__(kThreads, RB == 1 ? 4 : 2)
 few_layer_up_kernel(FewLayerArgs p, bool gated) {
   constexpr bool kFp8 = kIn != kHalf;
   constexpr int CT = 4, CS = kFp8 ? 2 : 1, KS = kWaves / CS, BN = 16 * CT * CS, kLd = BN + 4;
-  extern __shared__ __attribute__((aligned(16))) char s_raw[];
+  extern __shared__ __attribute__((aligned(16))) char s_all[];             // kQuantise: the rows' codes and scales first
   __shared__ Slots slots;
   const int T = p.tokens, n = T * p.k;
+  const RowsLds rows_at = rows_lds(kIn == kQuantise ? T : 0, p.d);
+  char *s_raw = s_all + rows_at.bytes;
+  if constexpr (kIn == kQuantise) quantise_here(p, s_all, rows_at);
   if (gated) {
     for (int q = threadIdx.x; q < n; q += kThreads) {
       const int64_t e = p.idx[q];
@@ -217,59 +313,45 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
     for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int b = 0; b < RB; ++b) acc[c][b] = float4v{0, 0, 0, 0};
-    int8v wf[2][CT], xf[2][RB], xw[2][RB];         // xw: the second half of 32 elements in 16 bits
+    int8v wf[2][CT], xf[2][RB];
     float sx[2][RB], sw[2];
-    auto fetch = [&](int q, auto B_) {             // the wavefront's step q; past the last one it again
+    auto fetch = [&](int q, auto B_) __attribute__((always_inline)) {      // the wavefront's step q; past the last one it again
       constexpr int buf = decltype(B_)::value;
       const int st = ks + (q < count ? q : count - 1) * KS;
 #pragma unroll
       for (int c = 0; c < CT; ++c) wf[buf][c] = piece(w[c], st * 128 + 32 * g, row_bytes);
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        if constexpr (kIn == kQuantise) {
-          const uint8_t *row = reinterpret_cast<const uint8_t *>(p.x + static_cast<size_t>(token[b]) * p.d);
-          xf[buf][b] = piece(row, st * 256 + 64 * g, 2 * p.d);
-          xw[buf][b] = piece(row, st * 256 + 64 * g + 32, 2 * p.d);
-        } else if constexpr (kIn == kCodes) {
+        if constexpr (kIn == kCodes) {
           xf[buf][b] = piece(p.x_codes + static_cast<size_t>(token[b]) * p.d, st * 128 + 32 * g, p.d);
           sx[buf][b] = p.x_scales[static_cast<size_t>(token[b]) * KB + st];
-        } else {
+        } else if constexpr (kIn == kHalf) {
           xf[buf][b] = piece(reinterpret_cast<const uint8_t *>(p.x + static_cast<size_t>(token[b]) * p.d), st * 128 + 32 * g, row_bytes);
         }
       }
       if constexpr (kFp8) sw[buf] = sb[st];
     };
-    auto multiply = [&](int q, auto B_) {
+    auto multiply = [&](int q, auto B_) __attribute__((always_inline)) {
       constexpr int buf = decltype(B_)::value;
-      if (q >= count) return;                      // uniform
+      if (q < count) {                             // uniform
+        const int st = ks + q * KS;
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        int8v x = xf[buf][b];
-        float s = 1.0f;
-        if constexpr (kIn == kQuantise) {
-          typedef _Float16 half16 __attribute__((ext_vector_type(16)));
-          const half16 lo = __builtin_bit_cast(half16, xf[buf][b]), hi = __builtin_bit_cast(half16, xw[buf][b]);
-          float top = 0.0f;
+        for (int b = 0; b < RB; ++b) {
+          float s = 1.0f;
+          if constexpr (kIn == kQuantise) {
+            const char *row = s_all + token[b] * rows_at.ld + st * 128 + 32 * g;
+            xf[buf][b] = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 16));
+            s = *reinterpret_cast<const float *>(s_all + rows_at.scales + 4 * (token[b] * KB + st));
+          } else if constexpr (kIn == kCodes) {
+            s = sx[buf][b];
+          }
+          if constexpr (kFp8) s *= sw[buf];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) top = fmaxf(top, fmaxf(fabsf(static_cast<float>(lo[j])), fabsf(static_cast<float>(hi[j]))));
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          float inverse;
-          s = block_scale(top, &inverse);
-          auto four = [&](const half16 &v, int j) {
-            return pack_fp8(static_cast<float>(v[j]) * inverse, static_cast<float>(v[j + 1]) * inverse,
-                            static_cast<float>(v[j + 2]) * inverse, static_cast<float>(v[j + 3]) * inverse);
-          };
-          x = int8v{four(lo, 0), four(lo, 4), four(lo, 8), four(lo, 12), four(hi, 0), four(hi, 4), four(hi, 8), four(hi, 12)};
-        } else if constexpr (kIn == kCodes) {
-          s = sx[buf][b];
-        }
-        if constexpr (kFp8) s *= sw[buf];
+          for (int c = 0; c < CT; ++c) {
+            const float4v part = product<kFp8>(wf[buf][c], xf[buf][b]);
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const float4v part = product<kFp8>(wf[buf][c], x);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[c][b][j] = kFp8 ? fmaf(part[j], s, acc[c][b][j]) : acc[c][b][j] + part[j];
+            for (int j = 0; j < 4; ++j) acc[c][b][j] = kFp8 ? fmaf(part[j], s, acc[c][b][j]) : acc[c][b][j] + part[j];
+          }
         }
       }
     };
@@ -339,16 +421,24 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
   }
 }
 
-// 16 columns of the output, all chosen experts; the wavefronts cut the experts' K among them.  A token's results of an
-// expert are scaled by its score (and the blocks' scales) as they are added.
-template <bool kFp8, int RB>
-__global__ void __launch_bounds__(kThreads, RB == 1 ? 4 : 2)
+// CW columns of the output, all chosen experts; the wavefronts cut the experts' K among them.  With CW < 16 the 16 rows of a
+// product are CW columns on 16 / CW steps of K at a time, each product with the tokens of one of them: a narrow tile loads as
+// many bytes as a wide one, and there are enough of them for the chip.  A token's results of an expert are scaled by its
+// score (and the blocks' scales) as they are added.
+//
+// Sixteen wavefronts to a workgroup, of which there is one on a CU; eight where a step has the fragments of several blocks of
+// tokens or steps, which need twice the registers.
+constexpr int down_waves(int RB, int CW) { return RB == 1 && CW == 16 ? 16 : 8; }
+
+template <bool kFp8, int RB, int CW>
+__global__ void __launch_bounds__(down_waves(RB, CW) * 64, down_waves(RB, CW) / 4)
 few_layer_down_kernel(FewLayerArgs p) {
-  constexpr int kUnroll = RB == 1 ? 3 : 2, kLd = 16 + 4;
+  constexpr int kDownWaves = down_waves(RB, CW), kLd = 16 + 4, KG = 16 / CW;
+  constexpr int kUnroll = RB * KG > 4 ? 1 : 2;     // items fetched at a time
   __shared__ Slots slots;
-  __shared__ float s_part[kWaves][16 * RB][kLd];
+  __shared__ float s_part[kDownWaves][16 * RB][kLd];
   const int T = p.tokens, n = T * p.k;
-  for (int q = threadIdx.x; q < n; q += kThreads) {
+  for (int q = threadIdx.x; q < n; q += kDownWaves * 64) {
     const int64_t e = p.idx[q];
     slots.e[q] = e >= 0 && e < p.E ? static_cast<int>(e) : p.E;
     slots.score[q] = static_cast<float>(p.score[q]);
@@ -356,12 +446,12 @@ few_layer_down_kernel(FewLayerArgs p) {
   __syncthreads();
   const int n_act = slots.build(n, p.k, p.E);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r16 = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
-  const int row_bytes = p.f * (kFp8 ? 1 : 2), steps = (row_bytes + 127) / 128;
+  const int r16 = lane & 15, g = lane >> 4, n0 = blockIdx.x * CW;
+  const int mine_k = g * 4 / CW;                   // of the KG steps, the one that this lane's results (rows 4 g ..) are of
+  const int row_bytes = p.f * (kFp8 ? 1 : 2), steps = (row_bytes + 128 * KG - 1) / (128 * KG);         // of KG blocks of 128 bytes
   const int KB = scale_blocks(p.f), NB = scale_blocks(p.d);
-  const int count = steps > wave ? (steps - wave + kWaves - 1) / kWaves : 0;           // of an expert: steps wave, wave + 8, ...
+  const int count = steps > wave ? (steps - wave + kDownWaves - 1) / kDownWaves : 0;   // of an expert: steps wave, wave + 16, ...
   const int total = count * n_act;
-  const int col = n0 + r16 < p.d ? n0 + r16 : p.d - 1;
   float4v acc[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) acc[b] = float4v{0, 0, 0, 0};
@@ -374,7 +464,7 @@ few_layer_down_kernel(FewLayerArgs p) {
   bool chose[RB], any[RB];                         // this lane's token did, one of the 16 did
   auto expert = [&]() __attribute__((always_inline)) {
     const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
-    w = static_cast<const uint8_t *>(p.w2) + (static_cast<size_t>(e) * p.d + col) * row_bytes;
+    w = static_cast<const uint8_t *>(p.w2) + (static_cast<size_t>(e) * p.d + n0 + r16 % CW) * row_bytes;
     if constexpr (kFp8) sb = p.s2 + (static_cast<size_t>(e) * NB + n0 / kScaleBlock) * KB;
     // lanes of tokens that did not choose it read a row of one that did
 #pragma unroll
@@ -391,7 +481,7 @@ few_layer_down_kernel(FewLayerArgs p) {
       if constexpr (kFp8) sh[b] = p.h_scales + r * KB;
     }
   };
-  int8v wf[2][kUnroll], hf[2][kUnroll][RB];
+  int8v wf[2][kUnroll], hf[2][kUnroll][RB][KG];
   float sf[2][kUnroll][RB];
   bool mine[2][kUnroll][RB];
   auto fetch = [&](int q, auto B_) __attribute__((always_inline)) {        // items q ...; past the last one nothing new
@@ -400,18 +490,20 @@ few_layer_down_kernel(FewLayerArgs p) {
     for (int u = 0; u < kUnroll; ++u) {
       if (q + u < total) {                         // uniform
         if (at == wave) expert();
-        wf[buf][u] = piece(w, at * 128 + 32 * g, row_bytes);
-        const float b_scale = kFp8 ? sb[at] : 1.0f;
+        wf[buf][u] = piece(w, (at * KG + r16 / CW) * 128 + 32 * g, row_bytes);
+        const int kb = at * KG + mine_k < KB ? at * KG + mine_k : KB - 1;
+        const float b_scale = kFp8 ? sb[kb] : 1.0f;
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
           mine[buf][u][b] = chose[b];
           sf[buf][u][b] = score[b];
           if (any[b]) {                            // uniform
-            hf[buf][u][b] = piece(h[b], at * 128 + 32 * g, row_bytes);
-            if constexpr (kFp8) sf[buf][u][b] *= sh[b][at] * b_scale;
+#pragma unroll
+            for (int j = 0; j < KG; ++j) hf[buf][u][b][j] = piece(h[b], (at * KG + j) * 128 + 32 * g, row_bytes);
+            if constexpr (kFp8) sf[buf][u][b] *= sh[b][kb] * b_scale;
           }
         }
-        at += kWaves;
+        at += kDownWaves;
         if (at >= steps) {
           at = wave;
           ++i;
@@ -426,7 +518,12 @@ few_layer_down_kernel(FewLayerArgs p) {
       if (q + u < total) {                         // uniform
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-          const float4v part = product<kFp8>(wf[buf][u], hf[buf][u][b]);
+          float4v part = product<kFp8>(wf[buf][u], hf[buf][u][b][0]);
+#pragma unroll
+          for (int j = 1; j < KG; ++j) {
+            const float4v other = product<kFp8>(wf[buf][u], hf[buf][u][b][j]);
+            part = mine_k == j ? other : part;
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[b][j] = mine[buf][u][b] ? fmaf(part[j], sf[buf][u][b], acc[b][j]) : acc[b][j];
         }
@@ -451,16 +548,17 @@ few_layer_down_kernel(FewLayerArgs p) {
 #pragma unroll
   for (int b = 0; b < RB; ++b) *reinterpret_cast<float4v *>(&s_part[wave][16 * b + r16][4 * g]) = acc[b];
   __syncthreads();
-  for (int o = threadIdx.x; o < T * 16; o += kThreads) {
-    const int t = o / 16, c = n0 + o % 16;
-    if (c >= p.d) continue;
+  for (int o = threadIdx.x; o < T * CW; o += kDownWaves * 64) {
+    const int t = o / CW, c = n0 + o % CW;         // (d is a multiple of 64)
     float v = 0.0f;
     for (int s = 0; s < p.k; ++s) {
       const int e = slots.e[t * p.k + s];
       if (e < p.E && p.b2) v = fmaf(slots.score[t * p.k + s], static_cast<float>(p.b2[static_cast<size_t>(e) * p.d + c]), v);
     }
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) v += s_part[x][t][o % 16];
+    for (int x = 0; x < kDownWaves; ++x)
+#pragma unroll
+      for (int j = 0; j < KG; ++j) v += s_part[x][t][j * CW + o % CW];
     p.out[static_cast<size_t>(t) * p.d + c] = static_cast<half_t>(v);
   }
 }
@@ -476,7 +574,8 @@ namespace {
 template <int kIn, int RB>
 int launch_up(const FewLayerArgs &p, bool gated, size_t gate_bytes, hipStream_t st) {
   constexpr int BN = kIn == kHalf ? 64 : 128, KS = kIn == kHalf ? 8 : 4;
-  const size_t part = sizeof(float) * KS * 16 * RB * (BN + 4), lds = gate_bytes > part ? gate_bytes : part;
+  const size_t part = sizeof(float) * KS * 16 * RB * (BN + 4);
+  const size_t lds = (gate_bytes > part ? gate_bytes : part) + (kIn == kQuantise ? rows_lds(p.tokens, p.d).bytes : rows_lds(0, p.d).bytes);
   auto kernel = few_layer_up_kernel<kIn, RB>;
   if (lds > 65536 - sizeof(Slots)) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -485,9 +584,18 @@ int launch_up(const FewLayerArgs &p, bool gated, size_t gate_bytes, hipStream_t 
   }
   const int n = p.tokens * p.k;
   const long long units = static_cast<long long>(p.E < n ? p.E : n) * ((p.f + BN - 1) / BN);
-  const int most = lds > 65536 || RB > 1 || kIn != kHalf ? 256 : 512;      // workgroups on the chip at once
+  const int most = lds + sizeof(Slots) > 80 * 1024 || RB > 1 ? 256 : 512;              // workgroups on the chip at once
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(units < most ? units : most)), dim3(kThreads), lds, st, p, gated);
   return check_launch("few_layer_up_kernel");
+}
+
+template <bool kFp8, int RB>
+int launch_down(const FewLayerArgs &p, hipStream_t st) {
+  // the widest tiles of which there are enough for the chip
+  const int cw = p.d >= 16 * 256 ? 16 : (p.d >= 8 * 256 ? 8 : 4);
+  auto kernel = cw == 16 ? few_layer_down_kernel<kFp8, RB, 16> : (cw == 8 ? few_layer_down_kernel<kFp8, RB, 8> : few_layer_down_kernel<kFp8, RB, 4>);
+  hipLaunchKernelGGL(kernel, dim3(p.d / cw), dim3(down_waves(RB, cw) * 64), 0, st, p);
+  return check_launch("few_layer_down_kernel");
 }
 
 template <int RB>
@@ -495,18 +603,22 @@ int launch_few_layer(const FewLayerArgs &p, bool fp8, bool gated, size_t gate_by
   const int rc = !fp8 ? launch_up<kHalf, RB>(p, gated, gate_bytes, st)
                       : (p.x_codes ? launch_up<kCodes, RB>(p, gated, gate_bytes, st) : launch_up<kQuantise, RB>(p, gated, gate_bytes, st));
   if (rc) return rc;
-  auto kernel = fp8 ? few_layer_down_kernel<true, RB> : few_layer_down_kernel<false, RB>;
-  hipLaunchKernelGGL(kernel, dim3((p.d + 15) / 16), dim3(kThreads), 0, st, p);
-  return check_launch("few_layer_down_kernel");
+  return fp8 ? launch_down<true, RB>(p, st) : launch_down<false, RB>(p, st);
 }
+
+// What the first kernel may keep in LDS beside its part sums (70 KB at most) and the slots.
+constexpr int kMaxGateLds = 64 * 1024, kMaxRowsLds = 72 * 1024;
 
 }  // namespace
 
+bool few_layer_quantises(int tokens, int d) { return rows_lds(tokens, d).bytes <= kMaxRowsLds; }
+
 int few_layer(const FewLayerArgs &p, bool fp8, ccf_stream_t stream) {
   const int nparts = (p.d + kPart - 1) / kPart;
-  const long long chains = static_cast<long long>(p.tokens) * p.E * nparts;
-  // gated in the first kernel: at most two chains to a thread, and operands that fit in LDS
-  const bool here = chains <= 2 * kThreads && gate_lds(p.tokens, p.E, nparts).bytes <= 128 * 1024;
+  const long long chains = static_cast<long long>(p.E) * nparts;
+  // gated in the first kernel: its expert rows in registers, at most two chains to a thread, and operands that fit in LDS
+  const bool here = chains <= kGateChains && p.tokens * chains <= 2 * kThreads &&
+                    gate_lds(p.tokens, p.E, nparts).bytes <= kMaxGateLds;
   if (!here) {
     int tokens_per_wg = 0;
     if (int rc = gate_forward(p.x, p.wg, p.bg, p.tokens, p.d, p.E, p.k, CCF_F16, p.idx, p.score, nullptr, stream, nullptr, 0,
