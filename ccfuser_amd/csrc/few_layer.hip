@@ -15,6 +15,8 @@
 // In 8 bits (e4m3, a scale per block of 128) rows of x are quantised where they are read, as ccf_quantize_rows does, and
 // the first kernel's workgroups have the 128 columns of a scale of h.  Wavefronts cut K among them and read straight from
 // memory, 16 rows of 128 consecutive bytes at a time, two steps ahead; their sums meet in LDS in a fixed order.
+// Workgroups start their sums at K places of their own, which go by the column: started together, they read the same bytes
+// of rows a power of two apart, and few of the memory's channels (XXX).
 #include "few_layer.h"
 #include "gate_select.h"
 #include "gelu.h"
@@ -35,9 +37,9 @@ enum { kHalf = 0, kCodes = 1, kQuantise = 2 };     // fp16 weights; e4m3 ones, w
 
 __device__ __forceinline__ int8v join(int4v lo, int4v hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
 
-// 16 columns (w) by 16 tokens (x) over the 128 bytes of a step, from zero.
+// 16 columns (w) by 16 tokens (x) over the 128 bytes of a step: in 8 bits from zero, since a scale follows, else onto c.
 template <bool kFp8>
-__device__ __forceinline__ float4v product(int8v w, int8v x) {
+__device__ __forceinline__ float4v product(int8v w, int8v x, float4v c = float4v{0, 0, 0, 0}) {
   if constexpr (kFp8) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, float4v{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
   } else {
@@ -45,16 +47,23 @@ __device__ __forceinline__ float4v product(int8v w, int8v x) {
     const half16 a = __builtin_bit_cast(half16, w), b = __builtin_bit_cast(half16, x);
     const half8 a0 = __builtin_shufflevector(a, a, 0, 1, 2, 3, 4, 5, 6, 7), a1 = __builtin_shufflevector(a, a, 8, 9, 10, 11, 12, 13, 14, 15);
     const half8 b0 = __builtin_shufflevector(b, b, 0, 1, 2, 3, 4, 5, 6, 7), b1 = __builtin_shufflevector(b, b, 8, 9, 10, 11, 12, 13, 14, 15);
-    const float4v c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b0, float4v{0, 0, 0, 0}, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b0, c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b1, c, 0, 0, 0);
   }
 }
 
-// 32 bytes of a row of `bytes` from byte `at` on; zeros behind its end.
-__device__ __forceinline__ int8v piece(const uint8_t *row, int at, int bytes) {
+// 32 bytes of a lane's row, whose byte `in_step` of step 0 lies at base + row; zeros behind the end of the row's `bytes`.  A
+// step is the 128 bytes (`span` times that) that the wavefront reads of every row; it and base are the wavefront's own.
+__device__ __forceinline__ int8v piece(const uint8_t *base, uint32_t row, int step, int in_step, int bytes, int span = 1) {
+  const uint8_t *at = base + step * 128;
+  if ((step + span) * 128 <= bytes) {
+    const int4v *both = reinterpret_cast<const int4v *>(at + (row + in_step));
+    return join(both[0], both[1]);
+  }
+  const int left = bytes - step * 128 - in_step;
   const int4v *zeros = &kZeros16;
-  const int4v *lo = at < bytes ? reinterpret_cast<const int4v *>(row + at) : zeros;
-  const int4v *hi = at + 16 < bytes ? reinterpret_cast<const int4v *>(row + at + 16) : zeros;
+  const int4v *lo = left > 0 ? reinterpret_cast<const int4v *>(at + (row + in_step)) : zeros;
+  const int4v *hi = left > 16 ? reinterpret_cast<const int4v *>(at + (row + in_step) + 16) : zeros;
   return join(*lo, *hi);
 }
 
@@ -127,6 +136,8 @@ __device__ __forceinline__ void gate_here(const FewLayerArgs &p, char *s_raw, Sl
       piece_of[s][i] = half8{0, 0, 0, 0, 0, 0, 0, 0};
       if (chain < chains && kk < d) piece_of[s][i] = *reinterpret_cast<const half8 *>(p.wg + static_cast<size_t>(e) * d + kk);
     }
+  float bias = 0.0f;                               // of the logit that this thread adds up
+  if (p.bg && static_cast<int>(threadIdx.x) < T * E) bias = static_cast<float>(p.bg[threadIdx.x - by_experts.div(threadIdx.x) * E]);
   const int x_pieces = T * nparts * 16;
 #pragma unroll 4
   for (int q = threadIdx.x; q < x_pieces; q += kThreads) {
@@ -183,25 +194,26 @@ __device__ __forceinline__ void gate_here(const FewLayerArgs &p, char *s_raw, Sl
   __syncthreads();
   for (int i = threadIdx.x; i < T * E; i += kThreads) {
     const float *ps = s_part + i * (nparts + 1);
-    float v = ps[0];
-#pragma unroll 8
-    for (int q = 1; q < nparts; ++q) v = v + ps[q];
     const int t = by_experts.div(i), e = i - t * E;
-    if (p.bg) v = v + static_cast<float>(p.bg[e]);
+    float v = ps[0];
+#pragma unroll 16
+    for (int q = 1; q < nparts; ++q) v = v + ps[q];
+    if (p.bg) v = v + (i < kThreads ? bias : static_cast<float>(p.bg[e]));
     s_logit[t * (E + 1) + e] = round_to<half_t>(v);
   }
   __syncthreads();
-  if (static_cast<int>(threadIdx.x) < T) {
+  auto select = [&](auto KS_) __attribute__((always_inline)) {
+    constexpr int KS = decltype(KS_)::value;       // most entries of a list
     const int t = threadIdx.x;
-    Best<kMaxTopK> best;
+    Best<KS> best;
     best.clear();
 #pragma unroll 8
     for (int e = 0; e < E; ++e) best.offer(s_logit[t * (E + 1) + e], e, k);
-    int64_t idx[kMaxTopK];
-    half_t score[kMaxTopK];
-    best.write<half_t>(0, k, idx, score);
+    int64_t idx[KS];
+    half_t score[KS];
+    best.template write<half_t>(0, k, idx, score);
 #pragma unroll
-    for (int s = 0; s < kMaxTopK; ++s)
+    for (int s = 0; s < KS; ++s)
       if (s < k) {
         slots.e[t * k + s] = best.id[s];
         if (blockIdx.x == 0) {                     // for the second kernel
@@ -209,6 +221,10 @@ __device__ __forceinline__ void gate_here(const FewLayerArgs &p, char *s_raw, Sl
           p.score[t * k + s] = score[s];
         }
       }
+  };
+  if (static_cast<int>(threadIdx.x) < T) {
+    if (k <= 2) select(std::integral_constant<int, 2>{});
+    else select(std::integral_constant<int, kMaxTopK>{});
   }
 }
 
@@ -265,7 +281,7 @@ __device__ __forceinline__ void quantise_here(const FewLayerArgs &p, char *s_row
 // 16 RB tokens; a workgroup's columns: 64 of fp16 weights, whose K all eight wavefronts cut among them, 128 in 8 bits, four
 // wavefronts to either half.
 template <int kIn, int RB>
-__global__ void __launch_bounds__(kThreads, RB == 1 ? 4 : 2)
+__global__ void __launch_bounds__(kThreads, RB == 1 && kIn != kCodes ? 4 : 2)
 few_layer_up_kernel(FewLayerArgs p, bool gated) {
   constexpr bool kFp8 = kIn != kHalf;
   constexpr int CT = 4, CS = kFp8 ? 2 : 1, KS = kWaves / CS, BN = 16 * CT * CS, kLd = BN + 4;
@@ -297,79 +313,104 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
   int token[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) token[b] = 16 * b + r16 < T ? 16 * b + r16 : T - 1;
+  const uint8_t *x = kIn == kCodes ? p.x_codes : reinterpret_cast<const uint8_t *>(p.x);
 
-  for (int u = blockIdx.x; u < n_act * blocks; u += gridDim.x) {
-    const int i = u / blocks, n0 = (u - i * blocks) * BN, c0 = n0 + cs * 16 * CT;
+  const int units = n_act * blocks;
+  if (static_cast<int>(blockIdx.x) >= units) return;
+  // a wavefront without a step takes part all the same: a step of another one's, not multiplied
+  const int turns = count > 0 ? count : 1;
+
+  // the item that is fetched next: the q-th of this wavefront's steps in unit u.  Its steps come in turn, from the one on
+  // that the unit's columns start at.
+  int u_next = blockIdx.x, q_next = 0, from_next = 0;
+  const uint8_t *w = nullptr;
+  const float *sb = nullptr;
+  auto aim = [&]() __attribute__((always_inline)) {
+    const int i = u_next / blocks, block = u_next - i * blocks;
+    int c0 = block * BN + cs * 16 * CT;
+    c0 = c0 < p.f ? c0 : p.f - 16 * CT;            // (f is a multiple of 64) the second half of 128 columns: never stored
     const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
-    const uint8_t *w[CT];
+    from_next = block % turns;
+    w = static_cast<const uint8_t *>(p.w1) + (static_cast<size_t>(e) * p.f + c0) * row_bytes;
+    if constexpr (kFp8) sb = p.s1 + (static_cast<size_t>(e) * FB + c0 / kScaleBlock) * KB;
+  };
+  auto step_of = [&](int from, int q) {
+    const int at = from + q, st = ks + (at < turns ? at : at - turns) * KS;
+    return st < steps ? st : steps - 1;
+  };
+  int8v wf[2][CT], xf[2][RB];
+  float sx[2][RB], sw[2];
+  auto fetch = [&](auto B_) __attribute__((always_inline)) {
+    constexpr int buf = decltype(B_)::value;
+    if (u_next >= units) return;                   // uniform
+    const int st = step_of(from_next, q_next);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      const int col = c0 + 16 * c + r16;
-      w[c] = static_cast<const uint8_t *>(p.w1) + (static_cast<size_t>(e) * p.f + (col < p.f ? col : p.f - 1)) * row_bytes;
+    for (int c = 0; c < CT; ++c) wf[buf][c] = piece(w + static_cast<size_t>(16 * c) * row_bytes, r16 * row_bytes, st, 32 * g, row_bytes);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      if constexpr (kIn == kCodes) {
+        xf[buf][b] = piece(x, token[b] * row_bytes, st, 32 * g, row_bytes);
+        sx[buf][b] = p.x_scales[token[b] * KB + st];
+      } else if constexpr (kIn == kHalf) {
+        xf[buf][b] = piece(x, token[b] * row_bytes, st, 32 * g, row_bytes);
+      }
     }
-    const float *sb = kFp8 ? p.s1 + (static_cast<size_t>(e) * FB + (c0 / kScaleBlock < FB ? c0 / kScaleBlock : FB - 1)) * KB : nullptr;
-    float4v acc[CT][RB];
+    if constexpr (kFp8) sw[buf] = sb[st];
+    if (++q_next == turns) {
+      q_next = 0;
+      u_next += gridDim.x;
+      if (u_next < units) aim();
+    }
+  };
+  // the unit that is computed, its item; eight consecutive columns of a token to a thread in its epilogue
+  constexpr int kPer = BN / 8;
+  static_assert(16 * RB * kPer <= kThreads, "a thread has at most one piece of the epilogue");
+  const int t_mine = threadIdx.x / kPer, c_mine = threadIdx.x % kPer * 8;
+  int u = blockIdx.x, q = 0, from = 0, i = 0, n0 = 0, slot = 255;
+  half8 bias;
+  float4v acc[CT][RB];
+  auto begin = [&]() __attribute__((always_inline)) {
+    i = u / blocks;
+    const int block = u - i * blocks, e = __builtin_amdgcn_readfirstlane(slots.act[i]);
+    from = block % turns;
+    n0 = block * BN;
+    slot = t_mine < T && n0 + c_mine < p.f ? slots.slot[i][t_mine] : 255;
+    bias = half8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (slot != 255 && p.b1) bias = *reinterpret_cast<const half8 *>(p.b1 + static_cast<size_t>(e) * p.f + n0 + c_mine);
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int b = 0; b < RB; ++b) acc[c][b] = float4v{0, 0, 0, 0};
-    int8v wf[2][CT], xf[2][RB];
-    float sx[2][RB], sw[2];
-    auto fetch = [&](int q, auto B_) __attribute__((always_inline)) {      // the wavefront's step q; past the last one it again
-      constexpr int buf = decltype(B_)::value;
-      const int st = ks + (q < count ? q : count - 1) * KS;
+  };
+  auto multiply = [&](auto B_) __attribute__((always_inline)) {
+    constexpr int buf = decltype(B_)::value;
+    if (count == 0) return;                        // uniform
+    const int st = step_of(from, q);
 #pragma unroll
-      for (int c = 0; c < CT; ++c) wf[buf][c] = piece(w[c], st * 128 + 32 * g, row_bytes);
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        if constexpr (kIn == kCodes) {
-          xf[buf][b] = piece(p.x_codes + static_cast<size_t>(token[b]) * p.d, st * 128 + 32 * g, p.d);
-          sx[buf][b] = p.x_scales[static_cast<size_t>(token[b]) * KB + st];
-        } else if constexpr (kIn == kHalf) {
-          xf[buf][b] = piece(reinterpret_cast<const uint8_t *>(p.x + static_cast<size_t>(token[b]) * p.d), st * 128 + 32 * g, row_bytes);
-        }
+    for (int b = 0; b < RB; ++b) {
+      float s = 1.0f;
+      if constexpr (kIn == kQuantise) {
+        const char *row = s_all + token[b] * rows_at.ld + st * 128 + 32 * g;
+        xf[buf][b] = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 16));
+        s = *reinterpret_cast<const float *>(s_all + rows_at.scales + 4 * (token[b] * KB + st));
+      } else if constexpr (kIn == kCodes) {
+        s = sx[buf][b];
       }
-      if constexpr (kFp8) sw[buf] = sb[st];
-    };
-    auto multiply = [&](int q, auto B_) __attribute__((always_inline)) {
-      constexpr int buf = decltype(B_)::value;
-      if (q < count) {                             // uniform
-        const int st = ks + q * KS;
+      if constexpr (kFp8) s *= sw[buf];
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          float s = 1.0f;
-          if constexpr (kIn == kQuantise) {
-            const char *row = s_all + token[b] * rows_at.ld + st * 128 + 32 * g;
-            xf[buf][b] = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 16));
-            s = *reinterpret_cast<const float *>(s_all + rows_at.scales + 4 * (token[b] * KB + st));
-          } else if constexpr (kIn == kCodes) {
-            s = sx[buf][b];
-          }
-          if constexpr (kFp8) s *= sw[buf];
+      for (int c = 0; c < CT; ++c) {
+        const float4v part = product<kFp8>(wf[buf][c], xf[buf][b], acc[c][b]);
+        if constexpr (kFp8) {
 #pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            const float4v part = product<kFp8>(wf[buf][c], xf[buf][b]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[c][b][j] = kFp8 ? fmaf(part[j], s, acc[c][b][j]) : acc[c][b][j] + part[j];
-          }
+          for (int j = 0; j < 4; ++j) acc[c][b][j] = fmaf(part[j], s, acc[c][b][j]);
+        } else {
+          acc[c][b] = part;
         }
-      }
-    };
-    if (count > 0) {
-      constexpr std::integral_constant<int, 0> even{};
-      constexpr std::integral_constant<int, 1> odd{};
-      fetch(0, even);
-      for (int q = 0; q < count; q += 2) {
-        fetch(q + 1, odd);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(q, even);
-        __builtin_amdgcn_sched_barrier(0);
-        fetch(q + 2, even);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(q + 1, odd);
-        __builtin_amdgcn_sched_barrier(0);
       }
     }
+  };
+  // the unit's end: the wavefronts' sums meet, GELU, h
+  auto finish = [&]() __attribute__((always_inline)) {
     __syncthreads();                               // the gate's or the last unit's LDS is read
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -377,47 +418,64 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
       for (int b = 0; b < RB; ++b)
         *reinterpret_cast<float4v *>(s_part + (ks * 16 * RB + 16 * b + r16) * kLd + (cs * CT + c) * 16 + 4 * g) = acc[c][b];
     __syncthreads();
-    // eight consecutive columns of a token to a thread
-    const half_t *bias = p.b1 ? p.b1 + static_cast<size_t>(e) * p.f : nullptr;
-    constexpr int kPer = BN / 8;
-    for (int o = threadIdx.x; o < 16 * RB * kPer; o += kThreads) {
-      const int t = o / kPer, c = (o % kPer) * 8, col = n0 + c;
-      const int slot = t < T ? slots.slot[i][t] : 255;
-      const bool mine = slot != 255 && col < p.f;
-      float v[8];
+    if (t_mine >= 16 * RB) return;
+    const bool mine = slot != 255;
+    float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = mine && bias ? static_cast<float>(bias[col + j]) : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(bias[j]);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const float *part = s_part + (s * 16 * RB + t) * kLd + c;
+    for (int s = 0; s < KS; ++s) {
+      const float *part = s_part + (s * 16 * RB + t_mine) * kLd + c_mine;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += part[j];
-      }
-      const size_t row = static_cast<size_t>(t) * p.k + (mine ? slot : 0);
-      float top = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = mine ? gelu_erf(v[j]) : 0.0f;
-        top = fmaxf(top, fabsf(v[j]));
-      }
-      if constexpr (kFp8) {
-#pragma unroll
-        for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        float inverse;
-        const float scale = block_scale(top, &inverse);
-        if (mine) {
-          if ((o & 15) == 0) p.h_scales[row * FB + col / kScaleBlock] = scale;
-          *reinterpret_cast<int2v *>(static_cast<uint8_t *>(p.h) + row * p.f + col) =
-              int2v{pack_fp8(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
-                    pack_fp8(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse)};
-        }
-      } else if (mine) {
-        half8 o8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o8[j] = static_cast<half_t>(v[j]);
-        *reinterpret_cast<half8 *>(static_cast<half_t *>(p.h) + row * p.f + col) = o8;
-      }
+      for (int j = 0; j < 8; ++j) v[j] += part[j];
     }
+    const size_t row = static_cast<size_t>(t_mine) * p.k + (mine ? slot : 0);
+    const int col = n0 + c_mine;
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = mine ? gelu_erf(v[j]) : 0.0f;
+      top = fmaxf(top, fabsf(v[j]));
+    }
+    if constexpr (kFp8) {
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+      float inverse;
+      const float scale = block_scale(top, &inverse);
+      if (mine) {
+        if (threadIdx.x % 16 == 0) p.h_scales[row * FB + col / kScaleBlock] = scale;
+        *reinterpret_cast<int2v *>(static_cast<uint8_t *>(p.h) + row * p.f + col) =
+            int2v{pack_fp8(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
+                  pack_fp8(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse)};
+      }
+    } else if (mine) {
+      half8 o8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o8[j] = static_cast<half_t>(v[j]);
+      *reinterpret_cast<half8 *>(static_cast<half_t *>(p.h) + row * p.f + col) = o8;
+    }
+  };
+  // one item, with the next one's loads (of the next unit, at a unit's end) on their way; whether it was the last
+  auto item = [&](auto B_) __attribute__((always_inline)) {
+    constexpr int buf = decltype(B_)::value;
+    fetch(std::integral_constant<int, buf ^ 1>{});
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(B_);
+    __builtin_amdgcn_sched_barrier(0);
+    if (++q < turns) return false;
+    finish();
+    q = 0;
+    u += gridDim.x;
+    if (u >= units) return true;
+    begin();
+    return false;
+  };
+  constexpr std::integral_constant<int, 0> even{};
+  constexpr std::integral_constant<int, 1> odd{};
+  aim();
+  fetch(even);
+  begin();
+  while (!item(even) && !item(odd)) {
   }
 }
 
@@ -457,14 +515,16 @@ few_layer_down_kernel(FewLayerArgs p) {
   for (int b = 0; b < RB; ++b) acc[b] = float4v{0, 0, 0, 0};
 
   // the item that is fetched next: step `at` of chosen expert `i`
-  int i = 0, at = wave;
-  const uint8_t *w = nullptr, *h[RB];
-  const float *sb = nullptr, *sh[RB];
+  const int from = count > 0 ? wave + blockIdx.x % count * kDownWaves : 0;
+  int i = 0, at = from;
+  const uint8_t *w = nullptr, *h = static_cast<const uint8_t *>(p.h);
+  const float *sb = nullptr;
+  uint32_t h_row[RB];
   float score[RB];
   bool chose[RB], any[RB];                         // this lane's token did, one of the 16 did
   auto expert = [&]() __attribute__((always_inline)) {
     const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
-    w = static_cast<const uint8_t *>(p.w2) + (static_cast<size_t>(e) * p.d + n0 + r16 % CW) * row_bytes;
+    w = static_cast<const uint8_t *>(p.w2) + (static_cast<size_t>(e) * p.d + n0) * row_bytes;
     if constexpr (kFp8) sb = p.s2 + (static_cast<size_t>(e) * NB + n0 / kScaleBlock) * KB;
     // lanes of tokens that did not choose it read a row of one that did
 #pragma unroll
@@ -475,12 +535,21 @@ few_layer_down_kernel(FewLayerArgs p) {
       any[b] = who != 0;
       const int row = chose[b] ? t * p.k + slot : 0;
       const int shared = __builtin_amdgcn_readlane(row, who ? __ffsll(who) - 1 : 0);
-      const size_t r = static_cast<size_t>(chose[b] ? row : shared);
+      h_row[b] = static_cast<uint32_t>(chose[b] ? row : shared);
       score[b] = chose[b] ? slots.score[row] : 0.0f;
-      h[b] = static_cast<const uint8_t *>(p.h) + r * row_bytes;
-      if constexpr (kFp8) sh[b] = p.h_scales + r * KB;
     }
   };
+  // the biases' part of this thread's output
+  const int t_mine = threadIdx.x / CW, c_mine = threadIdx.x % CW;
+  static_assert(16 * RB * CW <= kDownWaves * 64, "a thread has at most one output");
+  float sum = 0.0f;
+  if (p.b2 && t_mine < T) {
+#pragma unroll 2
+    for (int s = 0; s < p.k; ++s) {
+      const int e = slots.e[t_mine * p.k + s];
+      if (e < p.E) sum = fmaf(slots.score[t_mine * p.k + s], static_cast<float>(p.b2[static_cast<size_t>(e) * p.d + n0 + c_mine]), sum);
+    }
+  }
   int8v wf[2][kUnroll], hf[2][kUnroll][RB][KG];
   float sf[2][kUnroll][RB];
   bool mine[2][kUnroll][RB];
@@ -489,8 +558,8 @@ few_layer_down_kernel(FewLayerArgs p) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       if (q + u < total) {                         // uniform
-        if (at == wave) expert();
-        wf[buf][u] = piece(w, (at * KG + r16 / CW) * 128 + 32 * g, row_bytes);
+        if (at == from) expert();
+        wf[buf][u] = piece(w, r16 % CW * row_bytes, at * KG, r16 / CW * 128 + 32 * g, row_bytes, KG);
         const int kb = at * KG + mine_k < KB ? at * KG + mine_k : KB - 1;
         const float b_scale = kFp8 ? sb[kb] : 1.0f;
 #pragma unroll
@@ -499,15 +568,13 @@ few_layer_down_kernel(FewLayerArgs p) {
           sf[buf][u][b] = score[b];
           if (any[b]) {                            // uniform
 #pragma unroll
-            for (int j = 0; j < KG; ++j) hf[buf][u][b][j] = piece(h[b], (at * KG + j) * 128 + 32 * g, row_bytes);
-            if constexpr (kFp8) sf[buf][u][b] *= sh[b][kb] * b_scale;
+            for (int j = 0; j < KG; ++j) hf[buf][u][b][j] = piece(h, h_row[b] * row_bytes, at * KG + j, 32 * g, row_bytes);
+            if constexpr (kFp8) sf[buf][u][b] *= p.h_scales[h_row[b] * KB + kb] * b_scale;
           }
         }
         at += kDownWaves;
-        if (at >= steps) {
-          at = wave;
-          ++i;
-        }
+        if (at >= steps) at = wave;
+        if (at == from) ++i;
       }
     }
   };
@@ -548,18 +615,12 @@ few_layer_down_kernel(FewLayerArgs p) {
 #pragma unroll
   for (int b = 0; b < RB; ++b) *reinterpret_cast<float4v *>(&s_part[wave][16 * b + r16][4 * g]) = acc[b];
   __syncthreads();
-  for (int o = threadIdx.x; o < T * CW; o += kDownWaves * 64) {
-    const int t = o / CW, c = n0 + o % CW;         // (d is a multiple of 64)
-    float v = 0.0f;
-    for (int s = 0; s < p.k; ++s) {
-      const int e = slots.e[t * p.k + s];
-      if (e < p.E && p.b2) v = fmaf(slots.score[t * p.k + s], static_cast<float>(p.b2[static_cast<size_t>(e) * p.d + c]), v);
-    }
+  if (t_mine < T) {
 #pragma unroll
     for (int x = 0; x < kDownWaves; ++x)
 #pragma unroll
-      for (int j = 0; j < KG; ++j) v += s_part[x][t][j * CW + o % CW];
-    p.out[static_cast<size_t>(t) * p.d + c] = static_cast<half_t>(v);
+      for (int j = 0; j < KG; ++j) sum += s_part[x][t_mine][j * CW + c_mine];
+    p.out[static_cast<size_t>(t_mine) * p.d + n0 + c_mine] = static_cast<half_t>(sum);
   }
 }
 }  // namespace
@@ -584,7 +645,7 @@ int launch_up(const FewLayerArgs &p, bool gated, size_t gate_bytes, hipStream_t 
   }
   const int n = p.tokens * p.k;
   const long long units = static_cast<long long>(p.E < n ? p.E : n) * ((p.f + BN - 1) / BN);
-  const int most = lds + sizeof(Slots) > 80 * 1024 || RB > 1 ? 256 : 512;              // workgroups on the chip at once
+  const int most = lds + sizeof(Slots) > 80 * 1024 || RB > 1 || kIn == kCodes ? 256 : 512;              // workgroups on the chip at once
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(units < most ? units : most)), dim3(kThreads), lds, st, p, gated);
   return check_launch("few_layer_up_kernel");
 }
