@@ -52,18 +52,19 @@ __device__ __forceinline__ float4v product(int8v w, int8v x, float4v c = float4v
   }
 }
 
-// 32 bytes of a lane's row, whose byte `in_step` of step 0 lies at base + row; zeros behind the end of the row's `bytes`.  A
+// 32 bytes of a lane's row, 16 from byte `in_step` of the step on and 16 from 64 bytes further, so that the 4 lanes of a row
+// read 64 consecutive bytes at a time; zeros behind the end of the row's `bytes`, which begins at base + row.  A
 // step is the 128 bytes (`span` times that) that the wavefront reads of every row; it and base are the wavefront's own.
 __device__ __forceinline__ int8v piece(const uint8_t *base, uint32_t row, int step, int in_step, int bytes, int span = 1) {
   const uint8_t *at = base + step * 128;
   if ((step + span) * 128 <= bytes) {
     const int4v *both = reinterpret_cast<const int4v *>(at + (row + in_step));
-    return join(both[0], both[1]);
+    return join(both[0], both[4]);
   }
   const int left = bytes - step * 128 - in_step;
   const int4v *zeros = &kZeros16;
   const int4v *lo = left > 0 ? reinterpret_cast<const int4v *>(at + (row + in_step)) : zeros;
-  const int4v *hi = left > 16 ? reinterpret_cast<const int4v *>(at + (row + in_step) + 16) : zeros;
+  const int4v *hi = left > 64 ? reinterpret_cast<const int4v *>(at + (row + in_step) + 64) : zeros;
   return join(*lo, *hi);
 }
 
@@ -345,14 +346,14 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
     if (u_next >= units) return;                   // uniform
     const int st = step_of(from_next, q_next);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) wf[buf][c] = piece(w + static_cast<size_t>(16 * c) * row_bytes, r16 * row_bytes, st, 32 * g, row_bytes);
+    for (int c = 0; c < CT; ++c) wf[buf][c] = piece(w + static_cast<size_t>(16 * c) * row_bytes, r16 * row_bytes, st, 16 * g, row_bytes);
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       if constexpr (kIn == kCodes) {
-        xf[buf][b] = piece(x, token[b] * row_bytes, st, 32 * g, row_bytes);
+        xf[buf][b] = piece(x, token[b] * row_bytes, st, 16 * g, row_bytes);
         sx[buf][b] = p.x_scales[token[b] * KB + st];
       } else if constexpr (kIn == kHalf) {
-        xf[buf][b] = piece(x, token[b] * row_bytes, st, 32 * g, row_bytes);
+        xf[buf][b] = piece(x, token[b] * row_bytes, st, 16 * g, row_bytes);
       }
     }
     if constexpr (kFp8) sw[buf] = sb[st];
@@ -390,8 +391,8 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
     for (int b = 0; b < RB; ++b) {
       float s = 1.0f;
       if constexpr (kIn == kQuantise) {
-        const char *row = s_all + token[b] * rows_at.ld + st * 128 + 32 * g;
-        xf[buf][b] = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 16));
+        const char *row = s_all + token[b] * rows_at.ld + st * 128 + 16 * g;
+        xf[buf][b] = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 64));
         s = *reinterpret_cast<const float *>(s_all + rows_at.scales + 4 * (token[b] * KB + st));
       } else if constexpr (kIn == kCodes) {
         s = sx[buf][b];
@@ -559,7 +560,7 @@ few_layer_down_kernel(FewLayerArgs p) {
     for (int u = 0; u < kUnroll; ++u) {
       if (q + u < total) {                         // uniform
         if (at == from) expert();
-        wf[buf][u] = piece(w, r16 % CW * row_bytes, at * KG, r16 / CW * 128 + 32 * g, row_bytes, KG);
+        wf[buf][u] = piece(w, r16 % CW * row_bytes, at * KG, r16 / CW * 128 + 16 * g, row_bytes, KG);
         const int kb = at * KG + mine_k < KB ? at * KG + mine_k : KB - 1;
         const float b_scale = kFp8 ? sb[kb] : 1.0f;
 #pragma unroll
@@ -568,7 +569,7 @@ few_layer_down_kernel(FewLayerArgs p) {
           sf[buf][u][b] = score[b];
           if (any[b]) {                            // uniform
 #pragma unroll
-            for (int j = 0; j < KG; ++j) hf[buf][u][b][j] = piece(h, h_row[b] * row_bytes, at * KG + j, 32 * g, row_bytes);
+            for (int j = 0; j < KG; ++j) hf[buf][u][b][j] = piece(h, h_row[b] * row_bytes, at * KG + j, 16 * g, row_bytes);
             if constexpr (kFp8) sf[buf][u][b] *= p.h_scales[h_row[b] * KB + kb] * b_scale;
           }
         }
