@@ -133,12 +133,10 @@ struct FewWs {
   half_t *score;
   char *h;             // [n_flat, f] fp16, or codes
   float *h_scales;
-  uint8_t *x;          // codes [tokens, d] where the first kernel does not make them
-  float *x_scales;
   size_t total;
 };
 
-FewWs carve_few(void *ws, int tokens, int d, int f, int k, bool fp8) {
+FewWs carve_few(void *ws, int tokens, int f, int k, bool fp8) {
   const size_t n = static_cast<size_t>(tokens) * k;
   Carver c(ws);
   FewWs w;
@@ -146,8 +144,6 @@ FewWs carve_few(void *ws, int tokens, int d, int f, int k, bool fp8) {
   w.score = c.take<half_t>(n);
   w.h = c.take<char>(n * f * (fp8 ? 1 : 2));
   w.h_scales = c.take<float>(fp8 ? n * scale_blocks(f) : 0);
-  w.x = c.take<uint8_t>(fp8 ? static_cast<size_t>(tokens) * d : 0);
-  w.x_scales = c.take<float>(fp8 ? static_cast<size_t>(tokens) * scale_blocks(d) : 0);
   w.total = c.used;
   return w;
 }
@@ -428,7 +424,7 @@ extern "C" int ccf_moe_ffn_blocks(const void *x, int n_tokens, const int64_t *po
 
 extern "C" size_t ccf_moe_few_workspace_bytes(int tokens, int d_model, int d_ffn, int num_expert, int top_k) {
   if (!ccf::few_layer_fits(tokens, d_model, d_ffn, num_expert, top_k)) return 0;
-  return ccf::carve_few(nullptr, tokens, d_model, d_ffn, top_k, false).total;
+  return ccf::carve_few(nullptr, tokens, d_ffn, top_k, false).total;
 }
 
 extern "C" int ccf_moe_forward_few(const void *x, const void *wg, const void *bg, const void *w1, const void *b1, const void *w2,
@@ -447,7 +443,7 @@ extern "C" int ccf_moe_forward_few(const void *x, const void *wg, const void *bg
   const size_t need = ccf_moe_few_workspace_bytes(tokens, d_model, d_ffn, num_expert, top_k);
   CCF_REQUIRE(workspace && workspace_bytes >= need, CCF_ERR_WORKSPACE, "moe_forward_few: workspace of %zu bytes needed, %zu given",
               need, workspace_bytes);
-  FewWs w = carve_few(workspace, tokens, d_model, d_ffn, top_k, false);
+  FewWs w = carve_few(workspace, tokens, d_ffn, top_k, false);
   auto half = [](const void *p) { return static_cast<const half_t *>(p); };
   return few_layer(FewLayerArgs{half(x), nullptr, nullptr, half(wg), half(bg), w1, nullptr, half(b1), w2, nullptr, half(b2), tokens,
                                 d_model, d_ffn, num_expert, top_k, idx_out ? idx_out : w.idx,
@@ -459,7 +455,7 @@ extern "C" size_t ccf_moe_fp8_workspace_bytes(int tokens, int d_model, int d_ffn
   if (tokens < 0 || d_model <= 0 || d_ffn <= 0 || num_expert <= 0 || top_k <= 0) return 0;
   if (static_cast<long long>(tokens) * top_k >= (1ll << 31)) return 0;
   const size_t all = ccf::carve_moe8(nullptr, tokens, d_model, d_ffn, num_expert, top_k).total;
-  const size_t few = tokens <= 32 ? ccf::carve_few(nullptr, tokens, d_model, d_ffn, top_k, true).total : 0;
+  const size_t few = tokens <= 32 ? ccf::carve_few(nullptr, tokens, d_ffn, top_k, true).total : 0;
   return all > few ? all : few;
 }
 
@@ -487,13 +483,9 @@ extern "C" int ccf_moe_forward_fp8(const void *x, const void *x_codes, const flo
   auto bytes = [](const void *p) { return static_cast<const uint8_t *>(p); };
   hipStream_t st = as_stream(stream);
   // no expert can get more rows than there are tokens: a capacity of as many drops nothing
-  if (few_layer_fits(tokens, d_model, d_ffn, num_expert, top_k) && (capacity < 0 || capacity >= tokens)) {
-    FewWs w = carve_few(workspace, tokens, d_model, d_ffn, top_k, true);
-    if (!x_codes && !few_layer_quantises(tokens, d_model)) {
-      if (int rc = launch_quantize_rows(x, tokens, d_model, CCF_F16, w.x, w.x_scales, st)) return rc;
-      x_codes = w.x;
-      x_scales = w.x_scales;
-    }
+  if (few_layer_fits(tokens, d_model, d_ffn, num_expert, top_k) && few_layer_fits_fp8(tokens, d_model) &&
+      (capacity < 0 || capacity >= tokens)) {
+    FewWs w = carve_few(workspace, tokens, d_ffn, top_k, true);
     return few_layer(FewLayerArgs{half(x), bytes(x_codes), x_scales, half(wg), half(bg), w1_codes, w1_scales, half(b1), w2_codes,
                                   w2_scales, half(b2), tokens, d_model, d_ffn, num_expert, top_k, idx_out ? idx_out : w.idx,
                                   score_out ? static_cast<half_t *>(score_out) : w.score, w.h, w.h_scales, static_cast<half_t *>(out)},

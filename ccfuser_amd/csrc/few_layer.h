@@ -25,8 +25,8 @@ struct FewLayerArgs {
 };
 
 bool few_layer_fits(int tokens, int d, int f, int E, int k);
-// Whether the first kernel quantises the tokens for itself; otherwise the caller brings them in 8 bits.
-bool few_layer_quantises(int tokens, int d);
+// Whether the first kernel has room for the tokens in 8 bits.
+bool few_layer_fits_fp8(int tokens, int d);
 int few_layer(const FewLayerArgs &p, bool fp8, ccf_stream_t stream);
 
 }  // namespace ccf

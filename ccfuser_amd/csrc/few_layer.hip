@@ -33,8 +33,6 @@ constexpr int kThreads = 512, kWaves = kThreads / 64;
 
 __device__ const int4v kZeros16 = {0, 0, 0, 0};    // what lanes behind the end of K read
 
-enum { kHalf = 0, kCodes = 1, kQuantise = 2 };     // fp16 weights; e4m3 ones, with rows in 8 bits or quantised here into LDS
-
 __device__ __forceinline__ int8v join(int4v lo, int4v hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // 16 columns (w) by 16 tokens (x) over the 128 bytes of a step: in 8 bits from zero, since a scale follows, else onto c.
@@ -52,37 +50,26 @@ __device__ __forceinline__ float4v product(int8v w, int8v x, float4v c = float4v
   }
 }
 
-// 32 bytes of a lane's row, 16 from byte `in_step` of the step on and 16 from 64 bytes further, so that the 4 lanes of a row
-// read 64 consecutive bytes at a time; zeros behind the end of the row's `bytes`, which begins at base + row.  A
-// step is the 128 bytes (`span` times that) that the wavefront reads of every row; it and base are the wavefront's own.
-__device__ __forceinline__ int8v piece(const uint8_t *base, uint32_t row, int step, int in_step, int bytes, int span = 1) {
-  const uint8_t *at = base + step * 128;
-  if ((step + span) * 128 <= bytes) {
-    const int4v *both = reinterpret_cast<const int4v *>(at + (row + in_step));
-    return join(both[0], both[4]);
-  }
-  const int left = bytes - step * 128 - in_step;
-  const int4v *zeros = &kZeros16;
-  const int4v *lo = left > 0 ? reinterpret_cast<const int4v *>(at + (row + in_step)) : zeros;
-  const int4v *hi = left > 64 ? reinterpret_cast<const int4v *>(at + (row + in_step) + 64) : zeros;
-  return join(*lo, *hi);
-}
-
-// Which experts have tokens, in ascending order, and which slot of a token each is.
+// Which experts have tokens, in ascending order, and which slot of a token each is; in LDS.
 struct Slots {
-  unsigned mask[32];                               // of E <= 1024 experts
-  int act[kFewSlots];                              // the chosen experts
-  uint8_t slot[kFewSlots][kFewTokens];             // slot of token t that expert act[i] is, 255: none
-  int e[kFewSlots];                                // the tokens' choice
-  float score[kFewSlots];
+  unsigned *mask;                                  // [32] of E <= 1024 experts
+  int *act, *e;                                    // [n] the chosen experts; the tokens' choice
+  float *score;                                    // [n]
+  uint8_t *slot;                                   // [n][32] slot of token t that expert act[i] is, 255: none
 
+  __host__ __device__ static int bytes(int n) { return 128 + n * (4 + 4 + 4 + kFewTokens); }
+  __device__ __forceinline__ Slots(char *at, int n)
+      : mask(reinterpret_cast<unsigned *>(at)), act(reinterpret_cast<int *>(at + 128)), e(act + n),
+        score(reinterpret_cast<float *>(e + n)), slot(reinterpret_cast<uint8_t *>(score + n)) {}
+
+  __device__ __forceinline__ int of(int i, int t) const { return slot[i * kFewTokens + t]; }
   __device__ __forceinline__ int rank(int expert) const {
     int r = __popc(mask[expert >> 5] & ((1u << (expert & 31)) - 1));
     for (int i = 0; i < expert >> 5; ++i) r += __popc(mask[i]);
     return r;
   }
   // all threads, behind a barrier after e and score were written; how many experts were chosen
-  __device__ int build(int n, int k, int E) {
+  __device__ __forceinline__ int build(int n, int k, int E) {
     if (threadIdx.x < 32) mask[threadIdx.x] = 0;
     for (int i = threadIdx.x; i < n * kFewTokens / 4; i += blockDim.x) reinterpret_cast<unsigned *>(slot)[i] = 0xffffffffu;
     __syncthreads();
@@ -93,7 +80,7 @@ struct Slots {
     if (valid) {
       const int r = rank(mine), t = q / k;
       act[r] = mine;
-      slot[r][t] = static_cast<uint8_t>(q - t * k);
+      slot[r * kFewTokens + t] = static_cast<uint8_t>(q - t * k);
     }
     int total = 0;
     for (int i = 0; i < (E + 31) / 32; ++i) total += __popc(mask[i]);
@@ -101,6 +88,56 @@ struct Slots {
     return __builtin_amdgcn_readfirstlane(total);
   }
 };
+
+// ---- a wavefront's stream of operands
+//
+// Weights and tokens go to LDS by direct loads into a ring of the wavefront's own, kDepth items deep, each item the weights
+// (16 rows of 128 bytes: two loads of 8 whole lines) and the tokens of one product: no barrier, the wavefront waits for its
+// oldest item by the number of loads that may still be in flight.  16-byte chunk c of row r lies at c ^ (r % 8); a lane's
+// fragment is chunks g and g + 4 of row r16, of either operand.  (Loads into registers touch 64 bytes of 16 rows each:
+// 2 GiB of weights streamed that way came at 5.5 to 5.9 TB/s and, with the non-temporal hint, 5.2, whole lines with it at
+// 6.5 to 6.8.)
+//
+// The loads are asm for what the compiler does not know: which LDS reads they concern.  They write no register.
+template <bool kNT>
+__device__ __forceinline__ void load16_to_lds(const void *base, uint32_t offset, uint32_t at) {
+  if constexpr (kNT)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(at), "v"(offset), "s"(base));
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base));
+}
+__device__ __forceinline__ void load16_to_lds(const void *src, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src));
+}
+__device__ __forceinline__ void load4_to_lds(const void *base, uint32_t offset, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(at), "v"(offset), "s"(base));
+}
+// All but the newest n loads have landed.
+template <int n>
+__device__ __forceinline__ void loads_but() {
+  static_assert(n >= 0 && n < 64, "vmcnt has six bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (n & 15) | (n >> 4) << 14);
+  asm volatile("" ::: "memory");
+}
+// The LDS reads so far have their values: their place may be loaded into.
+__device__ __forceinline__ void reads_done() {
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char *)p));
+}
+__device__ __forceinline__ int8v fragment(const char *tile, int r, int g) {
+  const char *row = tile + r * 128;
+  return join(*reinterpret_cast<const int4v *>(row + ((g ^ (r & 7)) << 4)), *reinterpret_cast<const int4v *>(row + (((g ^ (r & 7)) ^ 4) << 4)));
+}
+__device__ __forceinline__ float scalar_load(const float *p) { return *(const __attribute__((address_space(4))) float *)p; }
+
+// Whether weights are loaded past the caches: where more passes before they are read again than the 256 MB Infinity Cache
+// holds (few.hip has the measurements).
+__device__ __forceinline__ bool pass_by(int n_act, int d, int f, bool fp8) {
+  return 2.0f * static_cast<float>(n_act) * static_cast<float>(d) * static_cast<float>(f) * (fp8 ? 1.0f : 2.0f) >= 320e6f;
+}
 
 // LDS of the gate: a slice of the expert rows (32 elements of every part), token rows, part sums, logits
 struct GateLds {
@@ -121,7 +158,7 @@ __host__ __device__ inline GateLds gate_lds(int T, int E, int nparts) {
 // ascending order, the bias last, one rounding to fp16.  The expert rows are loaded at once, 16 bytes at a time, into
 // registers and pass through LDS in four slices, so that they leave room for a second workgroup on the CU.  Token rows lie
 // in LDS in 16-byte pieces, piece c of part i at c ^ (i % 16), so that lanes on neighbouring parts read other banks.
-__device__ __forceinline__ void gate_here(const FewLayerArgs &p, char *s_raw, Slots &slots) {
+__device__ __forceinline__ void gate_here(const FewLayerArgs &p, char *s_raw, const Slots &slots) {
   const int T = p.tokens, d = p.d, E = p.E, k = p.k, nparts = (d + kPart - 1) / kPart, chains = E * nparts;
   const GateLds at = gate_lds(T, E, nparts);
   const FastDiv by_parts(nparts), by_chains(chains), by_experts(E);
@@ -241,11 +278,25 @@ __host__ __device__ inline RowsLds rows_lds(int T, int d) {
   return l;
 }
 
-// As ccf_quantize_rows: 16 lanes to a block of 128.  Codes behind the end of K are zeros.  The caller's barrier follows.
-__device__ __forceinline__ void quantise_here(const FewLayerArgs &p, char *s_rows, const RowsLds &at) {
+// The caller's codes, or as ccf_quantize_rows makes them, 16 lanes to a block of 128.  Codes behind the end of K are zeros.
+// The caller's barrier follows.
+__device__ __forceinline__ void rows_here(const FewLayerArgs &p, char *s_rows, const RowsLds &at) {
   const int blocks = scale_blocks(p.d);
   const FastDiv by_blocks(blocks);
   const int pieces = p.tokens * blocks * 16;
+  if (p.x_codes) {
+    const int chunks = blocks * 8;                 // of 16 bytes, to a row
+    const FastDiv by_chunks(chunks);
+#pragma unroll 4
+    for (int q = threadIdx.x; q < p.tokens * chunks; q += kThreads) {
+      const int t = by_chunks.div(q), c = (q - t * chunks) * 16;
+      int4v v = int4v{0, 0, 0, 0};
+      if (c < p.d) v = *reinterpret_cast<const int4v *>(p.x_codes + static_cast<size_t>(t) * p.d + c);
+      *reinterpret_cast<int4v *>(s_rows + t * at.ld + c) = v;
+    }
+    for (int q = threadIdx.x; q < p.tokens * blocks; q += kThreads) reinterpret_cast<float *>(s_rows + at.scales)[q] = p.x_scales[q];
+    return;
+  }
   constexpr int kAhead = 4;                        // loads on their way
   for (int q0 = threadIdx.x; q0 < pieces; q0 += kAhead * kThreads) {
     half8 v[kAhead];
@@ -279,19 +330,29 @@ __device__ __forceinline__ void quantise_here(const FewLayerArgs &p, char *s_row
   }
 }
 
-// 16 RB tokens; a workgroup's columns: 64 of fp16 weights, whose K all eight wavefronts cut among them, 128 in 8 bits, four
-// wavefronts to either half.
-template <int kIn, int RB>
-__global__ void __launch_bounds__(kThreads, RB == 1 && kIn != kCodes ? 4 : 2)
-few_layer_up_kernel(FewLayerArgs p, bool gated) {
-  constexpr bool kFp8 = kIn != kHalf;
-  constexpr int CT = 4, CS = kFp8 ? 2 : 1, KS = kWaves / CS, BN = 16 * CT * CS, kLd = BN + 4;
-  extern __shared__ __attribute__((aligned(16))) char s_all[];             // kQuantise: the rows' codes and scales first
-  __shared__ Slots slots;
+// RB blocks of 16 tokens, of which 8 NX are there.  A workgroup's columns: 16 of fp16 weights, whose K its eight wavefronts
+// cut among them, 128 in 8 bits, 16 to a wavefront: the columns of a scale of h.  It takes one such unit after the other, the
+// next one's operands on their way.
+template <bool kFp8, int RB, int NX>
+struct UpShape {
+  static constexpr int CS = kFp8 ? 8 : 1, KS = kWaves / CS, BN = 16 * CS, kLd = BN + 4;
+  static constexpr int kLoads = 2 + (kFp8 ? 0 : NX * RB), kItem = 1024 * kLoads, kDepth = kFp8 ? 4 : 2;
+  static constexpr int kRing = kWaves * kDepth * kItem, kPart = 4 * KS * 16 * RB * kLd;
+};
+
+template <bool kFp8, int RB, int NX>
+__global__ void __launch_bounds__(kThreads, 4)
+few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
+  using S = UpShape<kFp8, RB, NX>;
+  constexpr int KS = S::KS, BN = S::BN, kLd = S::kLd;
+  // the rings (first the gate's), part sums, slots, in 8 bits the tokens' codes and scales
+  extern __shared__ __attribute__((aligned(1024))) char s_all[];
   const int T = p.tokens, n = T * p.k;
-  const RowsLds rows_at = rows_lds(kIn == kQuantise ? T : 0, p.d);
-  char *s_raw = s_all + rows_at.bytes;
-  if constexpr (kIn == kQuantise) quantise_here(p, s_all, rows_at);
+  float *s_part = reinterpret_cast<float *>(s_all + ring_bytes);           // [KS][16 RB][kLd]
+  Slots slots(s_all + ring_bytes + S::kPart, n);
+  const RowsLds rows_at = rows_lds(kFp8 ? T : 0, p.d);
+  char *s_rows = s_all + ring_bytes + S::kPart + (Slots::bytes(n) + 15) / 16 * 16;
+  if constexpr (kFp8) rows_here(p, s_rows, rows_at);
   if (gated) {
     for (int q = threadIdx.x; q < n; q += kThreads) {
       const int64_t e = p.idx[q];
@@ -300,63 +361,70 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
       if (!valid && blockIdx.x == 0) p.idx[q] = -1;
     }
   } else {
-    gate_here(p, s_raw, slots);
+    gate_here(p, s_all, slots);
   }
   __syncthreads();
   const int n_act = slots.build(n, p.k, p.E);
 
-  float *s_part = reinterpret_cast<float *>(s_raw);                        // [KS][16 RB][kLd]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4, ks = wave % KS, cs = wave / KS;
-  const int row_bytes = p.d * (kFp8 ? 1 : 2), steps = (row_bytes + 127) / 128;
+  const int row_bytes = p.d * (kFp8 ? 1 : 2), steps = (row_bytes + 127) / 128, tail = row_bytes % 128;
   const int blocks = (p.f + BN - 1) / BN, KB = scale_blocks(p.d), FB = scale_blocks(p.f);
   const int count = steps > ks ? (steps - ks + KS - 1) / KS : 0;           // steps ks, ks + KS, ...
-  int token[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) token[b] = 16 * b + r16 < T ? 16 * b + r16 : T - 1;
-  const uint8_t *x = kIn == kCodes ? p.x_codes : reinterpret_cast<const uint8_t *>(p.x);
-
   const int units = n_act * blocks;
   if (static_cast<int>(blockIdx.x) >= units) return;
   // a wavefront without a step takes part all the same: a step of another one's, not multiplied
   const int turns = count > 0 ? count : 1;
+  const bool nt = pass_by(n_act, p.d, p.f, kFp8);
+  const char *ring = s_all + wave * (S::kDepth * S::kItem);
+  const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_address(ring));
 
-  // the item that is fetched next: the q-th of this wavefront's steps in unit u.  Its steps come in turn, from the one on
-  // that the unit's columns start at.
-  int u_next = blockIdx.x, q_next = 0, from_next = 0;
+  // this lane's loads: chunk (lane % 8) ^ (row % 8) of row 8 j + lane / 8 of a tile
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  const uint32_t w_lane = (lane >> 3) * row_bytes + chunk * 16;
+  uint32_t x_lane[RB * NX];
+#pragma unroll
+  for (int j = 0; j < RB * NX; ++j) {
+    const int t = 8 * j + (lane >> 3);             // (two blocks of tokens have all 16 each)
+    x_lane[j] = (t < T ? t : T - 1) * row_bytes + chunk * 16;
+  }
+
+  // the item that is loaded next: the q-th of this wavefront's steps in unit u.  Its steps come in turn, from the one on that
+  // the unit's columns start at.
+  int u_next = blockIdx.x, q_next = 0, from_next = 0, slot_next = 0, ahead = 0;
   const uint8_t *w = nullptr;
-  const float *sb = nullptr;
   auto aim = [&]() __attribute__((always_inline)) {
     const int i = u_next / blocks, block = u_next - i * blocks;
-    int c0 = block * BN + cs * 16 * CT;
-    c0 = c0 < p.f ? c0 : p.f - 16 * CT;            // (f is a multiple of 64) the second half of 128 columns: never stored
+    int c0 = block * BN + cs * 16;
+    c0 = c0 < p.f ? c0 : p.f - 16;                 // (f is a multiple of 64) the second half of 128 columns: never stored
     const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
     from_next = block % turns;
     w = static_cast<const uint8_t *>(p.w1) + (static_cast<size_t>(e) * p.f + c0) * row_bytes;
-    if constexpr (kFp8) sb = p.s1 + (static_cast<size_t>(e) * FB + c0 / kScaleBlock) * KB;
   };
   auto step_of = [&](int from, int q) {
     const int at = from + q, st = ks + (at < turns ? at : at - turns) * KS;
     return st < steps ? st : steps - 1;
   };
-  int8v wf[2][CT], xf[2][RB];
-  float sx[2][RB], sw[2];
-  auto fetch = [&](auto B_) __attribute__((always_inline)) {
-    constexpr int buf = decltype(B_)::value;
-    if (u_next >= units) return;                   // uniform
+  auto load_item = [&]() __attribute__((always_inline)) {
     const int st = step_of(from_next, q_next);
-#pragma unroll
-    for (int c = 0; c < CT; ++c) wf[buf][c] = piece(w + static_cast<size_t>(16 * c) * row_bytes, r16 * row_bytes, st, 16 * g, row_bytes);
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      if constexpr (kIn == kCodes) {
-        xf[buf][b] = piece(x, token[b] * row_bytes, st, 16 * g, row_bytes);
-        sx[buf][b] = p.x_scales[token[b] * KB + st];
-      } else if constexpr (kIn == kHalf) {
-        xf[buf][b] = piece(x, token[b] * row_bytes, st, 16 * g, row_bytes);
-      }
+    const uint8_t *base = w + st * 128, *base8 = base + static_cast<size_t>(8) * row_bytes;
+    uint32_t at = ring_at + slot_next * S::kItem, lane_at = w_lane;
+    // chunks behind the end of a row: its step's first one again, for codes that are zeros
+    if (tail && st == steps - 1) lane_at -= chunk * 16 >= tail ? chunk * 16 : 0;
+    if (nt) {
+      load16_to_lds<true>(base, lane_at, at);
+      load16_to_lds<true>(base8, lane_at, at + 1024);
+    } else {
+      load16_to_lds<false>(base, lane_at, at);
+      load16_to_lds<false>(base8, lane_at, at + 1024);
     }
-    if constexpr (kFp8) sw[buf] = sb[st];
+    if constexpr (!kFp8) {
+      const uint8_t *x = reinterpret_cast<const uint8_t *>(p.x) + st * 128;
+#pragma unroll
+      for (int j = 0; j < RB * NX; ++j) load16_to_lds<false>(x, x_lane[j], at + 2048 + 1024 * j);
+    }
+    ++ahead;
+    slot_next = slot_next + 1 < S::kDepth ? slot_next + 1 : 0;
     if (++q_next == turns) {
       q_next = 0;
       u_next += gridDim.x;
@@ -367,57 +435,28 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
   constexpr int kPer = BN / 8;
   static_assert(16 * RB * kPer <= kThreads, "a thread has at most one piece of the epilogue");
   const int t_mine = threadIdx.x / kPer, c_mine = threadIdx.x % kPer * 8;
-  int u = blockIdx.x, q = 0, from = 0, i = 0, n0 = 0, slot = 255;
+  int u = blockIdx.x, q = 0, from = 0, i = 0, n0 = 0, slot = 255, place = 0;
+  const float *sb = nullptr;
   half8 bias;
-  float4v acc[CT][RB];
+  float4v acc[RB];
   auto begin = [&]() __attribute__((always_inline)) {
     i = u / blocks;
     const int block = u - i * blocks, e = __builtin_amdgcn_readfirstlane(slots.act[i]);
     from = block % turns;
     n0 = block * BN;
-    slot = t_mine < T && n0 + c_mine < p.f ? slots.slot[i][t_mine] : 255;
+    if constexpr (kFp8) sb = p.s1 + (static_cast<size_t>(e) * FB + block) * KB;
+    slot = t_mine < T && n0 + c_mine < p.f ? slots.of(i, t_mine) : 255;
     bias = half8{0, 0, 0, 0, 0, 0, 0, 0};
     if (slot != 255 && p.b1) bias = *reinterpret_cast<const half8 *>(p.b1 + static_cast<size_t>(e) * p.f + n0 + c_mine);
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-      for (int b = 0; b < RB; ++b) acc[c][b] = float4v{0, 0, 0, 0};
-  };
-  auto multiply = [&](auto B_) __attribute__((always_inline)) {
-    constexpr int buf = decltype(B_)::value;
-    if (count == 0) return;                        // uniform
-    const int st = step_of(from, q);
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      float s = 1.0f;
-      if constexpr (kIn == kQuantise) {
-        const char *row = s_all + token[b] * rows_at.ld + st * 128 + 16 * g;
-        xf[buf][b] = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 64));
-        s = *reinterpret_cast<const float *>(s_all + rows_at.scales + 4 * (token[b] * KB + st));
-      } else if constexpr (kIn == kCodes) {
-        s = sx[buf][b];
-      }
-      if constexpr (kFp8) s *= sw[buf];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const float4v part = product<kFp8>(wf[buf][c], xf[buf][b], acc[c][b]);
-        if constexpr (kFp8) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[c][b][j] = fmaf(part[j], s, acc[c][b][j]);
-        } else {
-          acc[c][b] = part;
-        }
-      }
-    }
+    for (int b = 0; b < RB; ++b) acc[b] = float4v{0, 0, 0, 0};
   };
   // the unit's end: the wavefronts' sums meet, GELU, h
   auto finish = [&]() __attribute__((always_inline)) {
-    __syncthreads();                               // the gate's or the last unit's LDS is read
+    __syncthreads();                               // the last unit's part sums are read
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-        *reinterpret_cast<float4v *>(s_part + (ks * 16 * RB + 16 * b + r16) * kLd + (cs * CT + c) * 16 + 4 * g) = acc[c][b];
+    for (int b = 0; b < RB; ++b)
+      *reinterpret_cast<float4v *>(s_part + (ks * 16 * RB + 16 * b + r16) * kLd + cs * 16 + 4 * g) = acc[b];
     __syncthreads();
     if (t_mine >= 16 * RB) return;
     const bool mine = slot != 255;
@@ -456,51 +495,82 @@ few_layer_up_kernel(FewLayerArgs p, bool gated) {
       *reinterpret_cast<half8 *>(static_cast<half_t *>(p.h) + row * p.f + col) = o8;
     }
   };
-  // one item, with the next one's loads (of the next unit, at a unit's end) on their way; whether it was the last
-  auto item = [&](auto B_) __attribute__((always_inline)) {
-    constexpr int buf = decltype(B_)::value;
-    fetch(std::integral_constant<int, buf ^ 1>{});
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(B_);
-    __builtin_amdgcn_sched_barrier(0);
-    if (++q < turns) return false;
+
+  aim();
+#pragma unroll
+  for (int j = 0; j < S::kDepth; ++j)
+    if (u_next < units) load_item();
+  begin();
+  while (true) {
+    if (ahead == S::kDepth) loads_but<S::kLoads *(S::kDepth - 1)>();
+    else loads_but<0>();                           // the last items: none are loaded behind them
+    const char *at = ring + place * S::kItem;
+    place = place + 1 < S::kDepth ? place + 1 : 0;
+    const int st = step_of(from, q);
+    const int8v wf = fragment(at, r16, g);
+    int8v xf[RB];
+    float sx[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      if constexpr (kFp8) {
+        const int t = 16 * b + r16 < T ? 16 * b + r16 : T - 1;
+        const char *row = s_rows + t * rows_at.ld + st * 128 + 16 * g;
+        xf[b] = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 64));
+        sx[b] = *reinterpret_cast<const float *>(s_rows + rows_at.scales + 4 * (t * KB + st)) * scalar_load(sb + st);
+      } else {
+        xf[b] = fragment(at + 2048 + 1024 * NX * b, r16 & (8 * NX - 1), g);
+      }
+    }
+    reads_done();
+    --ahead;
+    if (u_next < units) load_item();
+    if (count > 0) {                               // uniform
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const float4v part = product<kFp8>(wf, xf[b], acc[b]);
+        if constexpr (kFp8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[b][j] = fmaf(part[j], sx[b], acc[b][j]);
+        } else {
+          acc[b] = part;
+        }
+      }
+    }
+    if (++q < turns) continue;
     finish();
     q = 0;
     u += gridDim.x;
-    if (u >= units) return true;
+    if (u >= units) return;
     begin();
-    return false;
-  };
-  constexpr std::integral_constant<int, 0> even{};
-  constexpr std::integral_constant<int, 1> odd{};
-  aim();
-  fetch(even);
-  begin();
-  while (!item(even) && !item(odd)) {
   }
 }
 
 // CW columns of the output, all chosen experts; the wavefronts cut the experts' K among them.  With CW < 16 the 16 rows of a
-// product are CW columns on 16 / CW steps of K at a time, each product with the tokens of one of them: a narrow tile loads as
-// many bytes as a wide one, and there are enough of them for the chip.  A token's results of an expert are scaled by its
-// score (and the blocks' scales) as they are added.
-//
-// Sixteen wavefronts to a workgroup, of which there is one on a CU; eight where a step has the fragments of several blocks of
-// tokens or steps, which need twice the registers.
-constexpr int down_waves(int RB, int CW) { return RB == 1 && CW == 16 ? 16 : 8; }
+// product are CW columns on KG = 16 / CW steps of K at a time, each product with the tokens of one of them: a narrow tile
+// loads as many bytes as a wide one, and there are enough of them for two workgroups on every CU.  A token's results of an
+// expert are scaled by its score (and the blocks' scales) as they are added.
+template <bool kFp8, int RB, int NX, int CW>
+struct DownShape {
+  static constexpr int KG = 16 / CW, kLd = 16 + 4;
+  static constexpr int kLoads = 2 + KG * NX * RB + (kFp8 ? 1 : 0), kItem = 1024 * (2 + KG * NX * RB) + (kFp8 ? 256 : 0);
+  static constexpr int kDepth = kItem <= 3 * 1024 ? 3 : 2;
+  static constexpr int kRing = kWaves * kDepth * kItem, kPart = 4 * kWaves * 16 * RB * kLd;
+};
 
-template <bool kFp8, int RB, int CW>
-__global__ void __launch_bounds__(down_waves(RB, CW) * 64, down_waves(RB, CW) / 4)
+template <bool kFp8, int RB, int NX, int CW>
+__global__ void __launch_bounds__(kThreads, 4)
 few_layer_down_kernel(FewLayerArgs p) {
-  constexpr int kDownWaves = down_waves(RB, CW), kLd = 16 + 4, KG = 16 / CW;
-  constexpr int kUnroll = RB * KG > 4 ? 1 : 2;     // items fetched at a time
-  __shared__ Slots slots;
-  __shared__ float s_part[kDownWaves][16 * RB][kLd];
+  using S = DownShape<kFp8, RB, NX, CW>;
+  constexpr int KG = S::KG, kLd = S::kLd;
+  extern __shared__ __attribute__((aligned(1024))) char s_all[];           // the rings, part sums, slots
   const int T = p.tokens, n = T * p.k;
-  for (int q = threadIdx.x; q < n; q += kDownWaves * 64) {
+  float *s_part = reinterpret_cast<float *>(s_all + S::kRing);             // [wavefronts][16 RB][kLd]
+  Slots slots(s_all + S::kRing + S::kPart, n);
+  for (int q = threadIdx.x; q < n; q += kThreads) {
     const int64_t e = p.idx[q];
+    const float score = static_cast<float>(p.score[q]);
     slots.e[q] = e >= 0 && e < p.E ? static_cast<int>(e) : p.E;
-    slots.score[q] = static_cast<float>(p.score[q]);
+    slots.score[q] = score;
   }
   __syncthreads();
   const int n_act = slots.build(n, p.k, p.E);
@@ -509,40 +579,15 @@ few_layer_down_kernel(FewLayerArgs p) {
   const int mine_k = g * 4 / CW;                   // of the KG steps, the one that this lane's results (rows 4 g ..) are of
   const int row_bytes = p.f * (kFp8 ? 1 : 2), steps = (row_bytes + 128 * KG - 1) / (128 * KG);         // of KG blocks of 128 bytes
   const int KB = scale_blocks(p.f), NB = scale_blocks(p.d);
-  const int count = steps > wave ? (steps - wave + kDownWaves - 1) / kDownWaves : 0;   // of an expert: steps wave, wave + 16, ...
+  const int count = steps > wave ? (steps - wave + kWaves - 1) / kWaves : 0;           // of an expert: steps wave, wave + 8, ...
   const int total = count * n_act;
-  float4v acc[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) acc[b] = float4v{0, 0, 0, 0};
+  const bool nt = pass_by(n_act, p.d, p.f, kFp8);
+  const char *ring = s_all + wave * (S::kDepth * S::kItem);
+  const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_address(ring));
 
-  // the item that is fetched next: step `at` of chosen expert `i`
-  const int from = count > 0 ? wave + blockIdx.x % count * kDownWaves : 0;
-  int i = 0, at = from;
-  const uint8_t *w = nullptr, *h = static_cast<const uint8_t *>(p.h);
-  const float *sb = nullptr;
-  uint32_t h_row[RB];
-  float score[RB];
-  bool chose[RB], any[RB];                         // this lane's token did, one of the 16 did
-  auto expert = [&]() __attribute__((always_inline)) {
-    const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
-    w = static_cast<const uint8_t *>(p.w2) + (static_cast<size_t>(e) * p.d + n0) * row_bytes;
-    if constexpr (kFp8) sb = p.s2 + (static_cast<size_t>(e) * NB + n0 / kScaleBlock) * KB;
-    // lanes of tokens that did not choose it read a row of one that did
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const int t = 16 * b + r16, slot = t < T ? slots.slot[i][t] : 255;
-      chose[b] = slot != 255;
-      const unsigned long long who = __ballot(chose[b]);
-      any[b] = who != 0;
-      const int row = chose[b] ? t * p.k + slot : 0;
-      const int shared = __builtin_amdgcn_readlane(row, who ? __ffsll(who) - 1 : 0);
-      h_row[b] = static_cast<uint32_t>(chose[b] ? row : shared);
-      score[b] = chose[b] ? slots.score[row] : 0.0f;
-    }
-  };
   // the biases' part of this thread's output
   const int t_mine = threadIdx.x / CW, c_mine = threadIdx.x % CW;
-  static_assert(16 * RB * CW <= kDownWaves * 64, "a thread has at most one output");
+  static_assert(16 * RB * CW <= kThreads, "a thread has at most one output");
   float sum = 0.0f;
   if (p.b2 && t_mine < T) {
 #pragma unroll 2
@@ -551,76 +596,159 @@ few_layer_down_kernel(FewLayerArgs p) {
       if (e < p.E) sum = fmaf(slots.score[t_mine * p.k + s], static_cast<float>(p.b2[static_cast<size_t>(e) * p.d + n0 + c_mine]), sum);
     }
   }
-  int8v wf[2][kUnroll], hf[2][kUnroll][RB][KG];
-  float sf[2][kUnroll][RB];
-  bool mine[2][kUnroll][RB];
-  auto fetch = [&](int q, auto B_) __attribute__((always_inline)) {        // items q ...; past the last one nothing new
-    constexpr int buf = decltype(B_)::value;
+
+  // this lane's loads: chunk (lane % 8) ^ (row % 8) of row 8 j + lane / 8 of a tile; of the weights' the row is column
+  // r % CW at step r / CW of the item's
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  uint32_t w_lane[2];
+  int w_behind[2];                                 // where the chunk lies in the item's bytes of the column
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (q + u < total) {                         // uniform
-        if (at == from) expert();
-        wf[buf][u] = piece(w, r16 % CW * row_bytes, at * KG, r16 / CW * 128 + 16 * g, row_bytes, KG);
-        const int kb = at * KG + mine_k < KB ? at * KG + mine_k : KB - 1;
-        const float b_scale = kFp8 ? sb[kb] : 1.0f;
+  for (int j = 0; j < 2; ++j) {
+    const int r = 8 * j + (lane >> 3);
+    w_behind[j] = r / CW * 128 + chunk * 16;
+    w_lane[j] = r % CW * row_bytes + w_behind[j];
+  }
+  // the item that is loaded next: step `at` of chosen expert `i`, a token that did not choose it taking a row of one that did
+  const int from = count > 0 ? wave + blockIdx.x % count * kWaves : 0;
+  int i_next = 0, at_next = from, slot_next = 0, ahead = 0;
+  const uint8_t *w = nullptr;
+  uint32_t h_lane[RB * NX], s_lane = 0;
+  auto aim = [&]() __attribute__((always_inline)) {
+    const int e = __builtin_amdgcn_readfirstlane(slots.act[i_next]);
+    w = static_cast<const uint8_t *>(p.w2) + (static_cast<size_t>(e) * p.d + n0) * row_bytes;
+    const int t32 = lane & 31, slot32 = t32 < T ? slots.of(i_next, t32) : 255;
+    const int row32 = t32 * p.k + slot32;
+    const int some = __builtin_amdgcn_readlane(row32, __ffsll(__ballot(slot32 != 255)) - 1);
+    auto row_of = [&](int t) {
+      const int slot = t < T ? slots.of(i_next, t) : 255;
+      return static_cast<uint32_t>(slot != 255 ? t * p.k + slot : some);
+    };
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          mine[buf][u][b] = chose[b];
-          sf[buf][u][b] = score[b];
-          if (any[b]) {                            // uniform
-#pragma unroll
-            for (int j = 0; j < KG; ++j) hf[buf][u][b][j] = piece(h, h_row[b] * row_bytes, at * KG + j, 16 * g, row_bytes);
-            if constexpr (kFp8) sf[buf][u][b] *= p.h_scales[h_row[b] * KB + kb] * b_scale;
-          }
-        }
-        at += kDownWaves;
-        if (at >= steps) at = wave;
-        if (at == from) ++i;
-      }
-    }
+    for (int j = 0; j < RB * NX; ++j) h_lane[j] = row_of(8 * j + (lane >> 3)) * row_bytes + chunk * 16;
+    if constexpr (kFp8) s_lane = row_of(lane % (16 * RB)) * KB;
   };
-  auto multiply = [&](int q, auto B_) __attribute__((always_inline)) {
-    constexpr int buf = decltype(B_)::value;
+  auto load_item = [&]() __attribute__((always_inline)) {
+    if (at_next == from) aim();
+    const uint8_t *base = w + static_cast<size_t>(at_next) * (128 * KG), *h = static_cast<const uint8_t *>(p.h) + at_next * (128 * KG);
+    const uint32_t at = ring_at + slot_next * S::kItem;
+    const int left = row_bytes - at_next * (128 * KG);         // bytes of a row from this item on
+    uint32_t lane_at[2] = {w_lane[0], w_lane[1]};
+    if (left < 128 * KG) {
+      // chunks behind the end of a row: the item's first one again, for activations that are zeros
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (q + u < total) {                         // uniform
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          float4v part = product<kFp8>(wf[buf][u], hf[buf][u][b][0]);
-#pragma unroll
-          for (int j = 1; j < KG; ++j) {
-            const float4v other = product<kFp8>(wf[buf][u], hf[buf][u][b][j]);
-            part = mine_k == j ? other : part;
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[b][j] = mine[buf][u][b] ? fmaf(part[j], sf[buf][u][b], acc[b][j]) : acc[b][j];
-        }
-      }
+      for (int j = 0; j < 2; ++j) lane_at[j] -= w_behind[j] >= left ? w_behind[j] : 0;
     }
+    if (nt) {
+      load16_to_lds<true>(base, lane_at[0], at);
+      load16_to_lds<true>(base, lane_at[1], at + 1024);
+    } else {
+      load16_to_lds<false>(base, lane_at[0], at);
+      load16_to_lds<false>(base, lane_at[1], at + 1024);
+    }
+#pragma unroll
+    for (int k = 0; k < KG; ++k)
+#pragma unroll
+      for (int j = 0; j < RB * NX; ++j) {
+        const uint32_t to = at + 2048 + 1024 * (k * RB * NX + j);
+        if (left < 128 * KG)
+          load16_to_lds(128 * k + chunk * 16 < left ? h + (128 * k + h_lane[j]) : reinterpret_cast<const uint8_t *>(&kZeros16), to);
+        else
+          load16_to_lds<false>(h + 128 * k, h_lane[j], to);
+      }
+    if constexpr (kFp8) {
+      // the scales of the tokens at the item's steps, token t at step k in lane 16 RB k + t
+      const int k = lane / (16 * RB) < KG ? lane / (16 * RB) : KG - 1, kb = at_next * KG + k < KB ? at_next * KG + k : KB - 1;
+      load4_to_lds(p.h_scales, 4 * (s_lane + kb), at + 1024 * (2 + KG * NX * RB));
+    }
+    ++ahead;
+    slot_next = slot_next + 1 < S::kDepth ? slot_next + 1 : 0;
+    at_next += kWaves;
+    if (at_next >= steps) at_next = wave;
+    if (at_next == from) ++i_next;
   };
+  static_assert(!kFp8 || 16 * RB * KG <= 64, "a lane per token and step");
+
+  // the item that is computed
+  int i = 0, at = from, place = 0;
+  const float *sb = nullptr;
+  float score[RB];
+  bool chose[RB];
+  float4v acc[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) acc[b] = float4v{0, 0, 0, 0};
   if (total > 0) {
-    constexpr std::integral_constant<int, 0> even{};
-    constexpr std::integral_constant<int, 1> odd{};
-    fetch(0, even);
-    for (int q = 0; q < total; q += 2 * kUnroll) {
-      fetch(q + kUnroll, odd);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(q, even);
-      __builtin_amdgcn_sched_barrier(0);
-      fetch(q + 2 * kUnroll, even);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(q + kUnroll, odd);
-      __builtin_amdgcn_sched_barrier(0);
+    int loaded = 0;
+#pragma unroll
+    for (int j = 0; j < S::kDepth; ++j)
+      if (loaded < total) {
+        load_item();
+        ++loaded;
+      }
+    for (int item = 0; item < total; ++item) {
+      if (at == from) {
+        const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
+        if constexpr (kFp8) sb = p.s2 + (static_cast<size_t>(e) * NB + n0 / kScaleBlock) * KB;
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          const int t = 16 * b + r16, slot = t < T ? slots.of(i, t) : 255;
+          chose[b] = slot != 255;
+          score[b] = chose[b] ? slots.score[t * p.k + slot] : 0.0f;
+        }
+      }
+      if (ahead == S::kDepth) loads_but<S::kLoads *(S::kDepth - 1)>();
+      else loads_but<0>();
+      const char *tile = ring + place * S::kItem;
+      place = place + 1 < S::kDepth ? place + 1 : 0;
+      const int8v wf = fragment(tile, r16, g);
+      int8v hf[RB][KG];
+      float s[RB];
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+#pragma unroll
+        for (int k = 0; k < KG; ++k)
+          hf[b][k] = fragment(tile + 2048 + 1024 * NX * (k * RB + b), r16 & (8 * NX - 1), g);
+        s[b] = score[b];
+        if constexpr (kFp8) {
+          // (weights' scales of all the item's steps, this lane's picked)
+          float scale = scalar_load(sb + at * KG);
+#pragma unroll
+          for (int k = 1; k < KG; ++k) {
+            const float other = scalar_load(sb + (at * KG + k < KB ? at * KG + k : KB - 1));
+            scale = mine_k == k ? other : scale;
+          }
+          s[b] *= *reinterpret_cast<const float *>(tile + 1024 * (2 + KG * NX * RB) + 4 * (16 * RB * mine_k + 16 * b + r16)) * scale;
+        }
+      }
+      reads_done();
+      --ahead;
+      if (loaded < total) {
+        load_item();
+        ++loaded;
+      }
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        float4v part = product<kFp8>(wf, hf[b][0]);
+#pragma unroll
+        for (int k = 1; k < KG; ++k) {
+          const float4v other = product<kFp8>(wf, hf[b][k]);
+          part = mine_k == k ? other : part;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[b][j] = chose[b] ? fmaf(part[j], s[b], acc[b][j]) : acc[b][j];
+      }
+      at += kWaves;
+      if (at >= steps) at = wave;
+      if (at == from) ++i;
     }
   }
 #pragma unroll
-  for (int b = 0; b < RB; ++b) *reinterpret_cast<float4v *>(&s_part[wave][16 * b + r16][4 * g]) = acc[b];
+  for (int b = 0; b < RB; ++b) *reinterpret_cast<float4v *>(s_part + (wave * 16 * RB + 16 * b + r16) * kLd + 4 * g) = acc[b];
   __syncthreads();
   if (t_mine < T) {
 #pragma unroll
-    for (int x = 0; x < kDownWaves; ++x)
+    for (int x = 0; x < kWaves; ++x)
 #pragma unroll
-      for (int j = 0; j < KG; ++j) sum += s_part[x][t_mine][j * CW + c_mine];
+      for (int j = 0; j < KG; ++j) sum += s_part[(x * 16 * RB + t_mine) * kLd + j * CW + c_mine];
     p.out[static_cast<size_t>(t_mine) * p.d + n0 + c_mine] = static_cast<half_t>(sum);
   }
 }
@@ -633,47 +761,70 @@ bool few_layer_fits(int tokens, int d, int f, int E, int k) {
 
 namespace {
 
-template <int kIn, int RB>
+template <typename K>
+int allow_lds(K kernel, size_t lds) {
+  if (lds <= 65536) return CCF_OK;
+  hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(lds));
+  return e == hipSuccess ? static_cast<int>(CCF_OK) : fail(CCF_ERR_HIP, "few_layer: LDS attribute: %s", hipGetErrorString(e));
+}
+
+template <bool kFp8, int RB, int NX>
 int launch_up(const FewLayerArgs &p, bool gated, size_t gate_bytes, hipStream_t st) {
-  constexpr int BN = kIn == kHalf ? 64 : 128, KS = kIn == kHalf ? 8 : 4;
-  const size_t part = sizeof(float) * KS * 16 * RB * (BN + 4);
-  const size_t lds = (gate_bytes > part ? gate_bytes : part) + (kIn == kQuantise ? rows_lds(p.tokens, p.d).bytes : rows_lds(0, p.d).bytes);
-  auto kernel = few_layer_up_kernel<kIn, RB>;
-  if (lds > 65536 - sizeof(Slots)) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(lds));
-    if (e != hipSuccess) return fail(CCF_ERR_HIP, "few_layer: LDS attribute: %s", hipGetErrorString(e));
-  }
+  using S = UpShape<kFp8, RB, NX>;
   const int n = p.tokens * p.k;
-  const long long units = static_cast<long long>(p.E < n ? p.E : n) * ((p.f + BN - 1) / BN);
-  const int most = lds + sizeof(Slots) > 80 * 1024 || RB > 1 || kIn == kCodes ? 256 : 512;              // workgroups on the chip at once
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(units < most ? units : most)), dim3(kThreads), lds, st, p, gated);
+  const size_t ring = gate_bytes > S::kRing ? (gate_bytes + 1023) / 1024 * 1024 : S::kRing;
+  const size_t lds = ring + S::kPart + (Slots::bytes(n) + 15) / 16 * 16 + (kFp8 ? rows_lds(p.tokens, p.d).bytes : 0);
+  auto kernel = few_layer_up_kernel<kFp8, RB, NX>;
+  if (int rc = allow_lds(kernel, lds)) return rc;
+  const long long units = static_cast<long long>(p.E < n ? p.E : n) * ((p.f + S::BN - 1) / S::BN);
+  const int most = lds > 80 * 1024 ? 256 : 512;                // workgroups on the chip at once
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(units < most ? units : most)), dim3(kThreads), lds, st, p, gated,
+                     static_cast<int>(ring));
   return check_launch("few_layer_up_kernel");
 }
 
-template <bool kFp8, int RB>
-int launch_down(const FewLayerArgs &p, hipStream_t st) {
-  // the widest tiles of which there are enough for the chip
-  const int cw = p.d >= 16 * 256 ? 16 : (p.d >= 8 * 256 ? 8 : 4);
-  auto kernel = cw == 16 ? few_layer_down_kernel<kFp8, RB, 16> : (cw == 8 ? few_layer_down_kernel<kFp8, RB, 8> : few_layer_down_kernel<kFp8, RB, 4>);
-  hipLaunchKernelGGL(kernel, dim3(p.d / cw), dim3(down_waves(RB, cw) * 64), 0, st, p);
+template <bool kFp8, int RB, int NX, int CW>
+int launch_down_at(const FewLayerArgs &p, hipStream_t st) {
+  using S = DownShape<kFp8, RB, NX, CW>;
+  const size_t lds = S::kRing + S::kPart + Slots::bytes(p.tokens * p.k);
+  auto kernel = few_layer_down_kernel<kFp8, RB, NX, CW>;
+  if (int rc = allow_lds(kernel, lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3(p.d / CW), dim3(kThreads), lds, st, p);
   return check_launch("few_layer_down_kernel");
 }
 
-template <int RB>
-int launch_few_layer(const FewLayerArgs &p, bool fp8, bool gated, size_t gate_bytes, hipStream_t st) {
-  const int rc = !fp8 ? launch_up<kHalf, RB>(p, gated, gate_bytes, st)
-                      : (p.x_codes ? launch_up<kCodes, RB>(p, gated, gate_bytes, st) : launch_up<kQuantise, RB>(p, gated, gate_bytes, st));
-  if (rc) return rc;
-  return fp8 ? launch_down<true, RB>(p, st) : launch_down<false, RB>(p, st);
+template <bool kFp8, int RB, int NX>
+int launch_down(const FewLayerArgs &p, hipStream_t st) {
+  // the widest tiles of which there are two for every CU; more tokens have items of their own size with wide ones
+  if constexpr (RB == 1 && NX == 1) {
+    if (p.d < 8 * 256) return launch_down_at<kFp8, RB, NX, 4>(p, st);
+  }
+  if constexpr (RB == 1) {
+    if (p.d < 16 * 512) return launch_down_at<kFp8, RB, NX, 8>(p, st);
+  }
+  return launch_down_at<kFp8, RB, NX, 16>(p, st);
 }
 
-// What the first kernel may keep in LDS beside its part sums (70 KB at most) and the slots.
-constexpr int kMaxGateLds = 64 * 1024, kMaxRowsLds = 72 * 1024;
+template <bool kFp8>
+int launch_few_layer(const FewLayerArgs &p, bool gated, size_t gate_bytes, hipStream_t st) {
+  auto run = [&](auto RB_, auto NX_) {
+    constexpr int RB = decltype(RB_)::value, NX = decltype(NX_)::value;
+    if (int rc = launch_up<kFp8, RB, NX>(p, gated, gate_bytes, st)) return rc;
+    return launch_down<kFp8, RB, NX>(p, st);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  return p.tokens <= 8 ? run(One{}, One{}) : (p.tokens <= 16 ? run(One{}, Two{}) : run(Two{}, Two{}));
+}
+
+// What the first kernel may keep in LDS of the gate's operands, and of tokens in 8 bits beside its rings, part sums (17 KB at
+// most) and slots (11 KB).
+constexpr int kMaxGateLds = 64 * 1024, kMaxRowsLds = 64 * 1024;
 
 }  // namespace
 
-bool few_layer_quantises(int tokens, int d) { return rows_lds(tokens, d).bytes <= kMaxRowsLds; }
+bool few_layer_fits_fp8(int tokens, int d) { return rows_lds(tokens, d).bytes <= kMaxRowsLds; }
 
 int few_layer(const FewLayerArgs &p, bool fp8, ccf_stream_t stream) {
   const int nparts = (p.d + kPart - 1) / kPart;
@@ -688,8 +839,8 @@ int few_layer(const FewLayerArgs &p, bool fp8, ccf_stream_t stream) {
       return rc;
   }
   const size_t gate_bytes = here ? gate_lds(p.tokens, p.E, nparts).bytes : 0;
-  return p.tokens > 16 ? launch_few_layer<2>(p, fp8, !here, gate_bytes, as_stream(stream))
-                       : launch_few_layer<1>(p, fp8, !here, gate_bytes, as_stream(stream));
+  return fp8 ? launch_few_layer<true>(p, !here, gate_bytes, as_stream(stream))
+             : launch_few_layer<false>(p, !here, gate_bytes, as_stream(stream));
 }
 
 }  // namespace ccf
