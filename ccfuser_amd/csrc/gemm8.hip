@@ -135,14 +135,20 @@ __device__ __forceinline__ void load4_to_lds(const void *src, uint32_t at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(src));
 }
 
-// The experts' tiles in LDS, for a workgroup that runs several: first[e] tiles of rows in front of expert e's, first row of it.
+// Rows of an expert beyond its 256-row tiles cost as much as a whole one however few they are: up to kLeftRows of them may
+// go to a launch of smaller tiles.
+enum { kAll = 0, kWhole = 1, kLeft = 2 };            // all rows; without those; those alone
+constexpr int kWholeRows = 256, kLeftRows = 64;
+
+// The experts' tiles in LDS, for a workgroup that runs several: first[e] tiles of rows in front of expert e's, the first row
+// of it and, E further, the one behind its last.
 template <int BM>
 struct TileMap {
-  const int *first, *row;    // [E + 1] each
+  const int *first, *row;    // [E + 1], [2 E]
   int E, n_tiles;
 
-  // all threads; the caller's barrier follows
-  __device__ __forceinline__ static void build(const Gemm8Args &p, int *first, int *row) {
+  // all threads; the caller's barrier follows.  Of every expert's rows those that `part` says
+  __device__ __forceinline__ static void build(const Gemm8Args &p, int part, int *first, int *row) {
     if (threadIdx.x >= 64) return;
     const int lane = threadIdx.x;
     int before = 0;
@@ -153,6 +159,10 @@ struct TileMap {
         hi = p.offsets ? p.offsets[e0 + lane + 1] : p.max_rows;
         lo = lo < p.max_rows ? lo : p.max_rows;
         hi = hi < p.max_rows ? hi : p.max_rows;
+        const int over = hi > lo ? (hi - lo) % kWholeRows : 0;
+        const bool few = over <= kLeftRows;          // rows beyond whole tiles that tiles of their own take
+        if (part == kWhole && few) hi -= over;
+        if (part == kLeft) lo = few ? hi - over : hi;
       }
       int upto = hi > lo ? (hi - lo + BM - 1) / BM : 0;
 #pragma unroll
@@ -161,9 +171,10 @@ struct TileMap {
         upto += lane >= o ? v : 0;
       }
       if (e0 + lane < p.E) {
-        if (e0 + lane == 0) first[0] = 0, row[0] = lo;
+        if (e0 + lane == 0) first[0] = 0;
         first[e0 + lane + 1] = before + upto;
-        row[e0 + lane + 1] = hi;
+        row[e0 + lane] = lo;
+        row[p.E + e0 + lane] = hi;
       }
       before += __builtin_amdgcn_readlane(upto, 63);
     }
@@ -190,7 +201,7 @@ struct TileMap {
     r.n = in / gm;
     r.m = group * 8 + in - r.n * gm;
     r.row0 = __builtin_amdgcn_readfirstlane(row[e]) + r.m * BM;
-    r.rows = __builtin_amdgcn_readfirstlane(row[e + 1]) - r.row0;
+    r.rows = __builtin_amdgcn_readfirstlane(row[E + e]) - r.row0;
     return r;
   }
 };
@@ -239,12 +250,12 @@ __device__ __forceinline__ void tile_sources(const Gemm8Args &p, const Tile &til
 // tile's first loads are on their way while this one's last products and its epilogue run.
 template <int BM, int BN, int WM, int WN, int kOut>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
-gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
+gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
   using S = TileShape<BM, BN, WM, WN>;
   using Out = std::conditional_t<kOut == kGemm8Bf16, bf16_t, half_t>;
   extern __shared__ __attribute__((aligned(1024))) char s_tile[];          // two places, then the tile map
   int *s_map = reinterpret_cast<int *>(s_tile + 2 * S::kStage);
-  TileMap<BM>::build(p, s_map, s_map + p.E + 1);
+  TileMap<BM>::build(p, part, s_map, s_map + p.E + 1);
   __syncthreads();
   const TileMap<BM> map{s_map, s_map + p.E + 1, p.E, n_tiles};
   // workgroup ids go round the 8 XCDs: each XCD takes a run of tiles, which share operands in its L2
@@ -273,11 +284,11 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
   constexpr int kParts = 4;
   constexpr std::integral_constant<int, 0> kFirst{};
   auto load_part = [&](int place, auto PART) __attribute__((always_inline)) {
-    constexpr int part = decltype(PART)::value;
+    constexpr int quarter = decltype(PART)::value;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds + place * S::kStage + wave * 1024);
     const uint8_t *a = p.a + next_kb * kScaleBlock;
     const uint8_t *b = p.b + static_cast<size_t>(next.e) * p.N * p.K + next_kb * kScaleBlock;
-    constexpr int lo = part * S::kLoads / kParts, hi = (part + 1) * S::kLoads / kParts;
+    constexpr int lo = quarter * S::kLoads / kParts, hi = (quarter + 1) * S::kLoads / kParts;
     if (tail && next_kb == KB - 1) {
       // chunks behind the end of K: zeros for the rows, and for the columns the block's first chunk again (what is no
       // number there is no number in the sum anyway)
@@ -295,7 +306,7 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
         else load16_to_lds(b, src[i], at + i * S::kWaves * 1024);
       }
     }
-    if (part == 0 && (scales_of_rows || scales_of_columns))          // the wavefronts' 64 scales each, one behind the other
+    if (quarter == 0 && (scales_of_rows || scales_of_columns))          // the wavefronts' 64 scales each, one behind the other
       load4_to_lds(scale_base + next_kb + scale_src,
                    __builtin_amdgcn_readfirstlane(lds + place * S::kStage + S::kRowsBytes + wave * 256));
   };
@@ -307,7 +318,7 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
     return join(*reinterpret_cast<const int4v *>(place + at + i * 16 * kScaleBlock),
                 *reinterpret_cast<const int4v *>(place + (at ^ 64) + i * 16 * kScaleBlock));
   };
-  float4v acc[S::CT][S::TT], part[S::TT];
+  float4v acc[S::CT][S::TT], product[S::TT];
   int8v x[S::TT], w[2];
   float sa[S::TT], sb, s[S::TT];                     // scales as read for the coming step; of the step whose results are scaled
   auto clear = [&]() __attribute__((always_inline)) {
@@ -316,11 +327,11 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
 #pragma unroll
       for (int t = 0; t < S::TT; ++t) acc[c][t] = float4v{0, 0, 0, 0};
 #pragma unroll
-    for (int t = 0; t < S::TT; ++t) part[t] = float4v{0, 0, 0, 0}, s[t] = 0.0f;
+    for (int t = 0; t < S::TT; ++t) product[t] = float4v{0, 0, 0, 0}, s[t] = 0.0f;
   };
   auto scaled = [&](int c, int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[c][t][i] = fmaf(part[t][i], s[t], acc[c][t][i]);
+    for (int i = 0; i < 4; ++i) acc[c][t][i] = fmaf(product[t][i], s[t], acc[c][t][i]);
   };
   // the sums of columns c exist here: without that the compiler puts all scalings of a step off behind its branch, and
   // keeps their inputs in registers that there are not
@@ -359,14 +370,14 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
       w[(c + 1) & 1] = fragment(now, w_at, c + 1);
 #pragma unroll
       for (int t = 0; t < S::TT - 1; ++t) {
-        part[t] = mfma8(w[c & 1], x[t]);
+        product[t] = mfma8(w[c & 1], x[t]);
         scaled(c_before, t + 1);
       }
       if constexpr (c == 0) {
 #pragma unroll
         for (int t = 0; t < S::TT; ++t) s[t] = sa[t] * sb;
       }
-      part[S::TT - 1] = mfma8(w[c & 1], x[S::TT - 1]);
+      product[S::TT - 1] = mfma8(w[c & 1], x[S::TT - 1]);
       scaled(c, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
@@ -397,7 +408,7 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles) {
     const char *ahead = s_tile + (place ^ 1) * S::kStage;            // behind the last step: read for nothing
 #pragma unroll
     for (int t = 0; t < S::TT; ++t) {
-      part[t] = mfma8(w[last & 1], x[t]);
+      product[t] = mfma8(w[last & 1], x[t]);
       if (t + 1 < S::TT) scaled(last - 1, t + 1);
       else scaled(last, 0);
       x[t] = fragment(ahead, x_at, t);
@@ -656,20 +667,10 @@ long long grid_of(const Gemm8Args &p, int bm, int n_tiles) {
   return (m * n_tiles + 7) / 8 * 8;
 }
 
-template <typename K>
-int launch(K kernel, const Gemm8Args &p, int bm, int bn, int threads, size_t lds, long long most, hipStream_t st,
-           const char *what) {
-  const int n_tiles = (p.N + bn - 1) / bn;
-  long long grid = grid_of(p, bm, n_tiles);
-  CCF_REQUIRE(grid < (1ll << 28), CCF_ERR_SHAPE, "%s: too many tiles", what);
-  grid = grid < most ? grid : most;
-  if (lds > 65536) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(lds));
-    if (e != hipSuccess) return fail(CCF_ERR_HIP, "%s: LDS attribute: %s", what, hipGetErrorString(e));
-  }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), lds, st, p, n_tiles);
-  return check_launch(what);
+int allow_lds(const void *kernel, size_t lds, const char *what) {
+  if (lds <= 65536) return CCF_OK;
+  hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+  return e == hipSuccess ? static_cast<int>(CCF_OK) : fail(CCF_ERR_HIP, "%s: LDS attribute: %s", what, hipGetErrorString(e));
 }
 
 // Compute units of the current device, in whole rounds of the 8 XCDs.
@@ -687,17 +688,29 @@ int compute_units() {
 }
 
 template <int BM, int BN, int WM, int WN, int kOut>
-int launch_tiles(const Gemm8Args &p, hipStream_t st, const char *what) {
+int launch_tiles(const Gemm8Args &p, int part, hipStream_t st, const char *what) {
   using S = TileShape<BM, BN, WM, WN>;
-  const int cus = compute_units();
+  auto kernel = gemm8_tile_kernel<BM, BN, WM, WN, kOut>;
+  const size_t lds = 2 * S::kStage + 4 * (3 * p.E + 1);
+  const int cus = compute_units(), n_tiles = (p.N + BN - 1) / BN;
   CCF_REQUIRE(cus > 0, CCF_ERR_HIP, "%s: no device", what);
-  return launch(gemm8_tile_kernel<BM, BN, WM, WN, kOut>, p, BM, BN, S::kThreads, 2 * S::kStage + 8 * (p.E + 1), cus, st, what);
+  if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), lds, what)) return rc;
+  const long long tiles = part == kLeft ? (static_cast<long long>(n_tiles) * (p.offsets ? p.E : 1) + 7) / 8 * 8 : grid_of(p, BM, n_tiles);
+  const long long most = static_cast<long long>(cus) * (160 * 1024 / lds);             // workgroups on the chip at once
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles < most ? tiles : most)), dim3(S::kThreads), lds, st, p, n_tiles, part);
+  return check_launch(what);
 }
 
 template <int TT, int CT, int CS, int kOut>
 int launch_split(const Gemm8Args &p, hipStream_t st, const char *what) {
   using S = SplitShape<TT, CT, CS>;
-  return launch(gemm8_split_kernel<TT, CT, CS, kOut>, p, S::BM, S::BN, 512, S::kLds, 1ll << 28, st, what);
+  auto kernel = gemm8_split_kernel<TT, CT, CS, kOut>;
+  const int n_tiles = (p.N + S::BN - 1) / S::BN;
+  const long long grid = grid_of(p, S::BM, n_tiles);
+  CCF_REQUIRE(grid < (1ll << 28), CCF_ERR_SHAPE, "%s: too many tiles", what);
+  if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), S::kLds, what)) return rc;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(512), S::kLds, st, p, n_tiles);
+  return check_launch(what);
 }
 
 template <int kOut>
@@ -707,12 +720,19 @@ int gemm8_out(const Gemm8Args &p, hipStream_t st, const char *what) {
   // (the 8-bit output wants all 128 columns of a scale in one workgroup)
   constexpr int CS = kOut == kGemm8Gelu8 ? 2 : 1;
   const bool can_tile = p.K > kScaleBlock;                     // two steps at least
-  if (g_fp8_form == 2 && can_tile) return launch_tiles<256, 256, 4, 2, kOut>(p, st, what);
-  if (rows <= 16) return launch_split<1, 4, CS, kOut>(p, st, what);
-  if (rows <= 32) return launch_split<2, 4, CS, kOut>(p, st, what);
+  int form = g_fp8_form;
   const long long large = static_cast<long long>(p.max_rows / 256 + owners) * ((p.N + 255) / 256);
-  if (g_fp8_form == 1 || !can_tile || rows <= 128 || large < 256) return launch_split<4, 4, 2, kOut>(p, st, what);
-  return launch_tiles<256, 256, 4, 2, kOut>(p, st, what);
+  if (form == 0) form = !can_tile || rows <= 32 ? 1 : (rows > 128 && large >= 256 ? 2 : (rows > 64 ? 3 : 4));
+  if (!can_tile) form = 1;
+  if (form == 1) {
+    if (rows <= 16) return launch_split<1, 4, CS, kOut>(p, st, what);
+    return launch_split<2, 4, CS, kOut>(p, st, what);
+  }
+  if (form == 2) return launch_tiles<256, 256, 4, 2, kOut>(p, kAll, st, what);
+  if (form == 3) return launch_tiles<128, 128, 4, 1, kOut>(p, kAll, st, what);
+  if (form == 4) return launch_tiles<64, 128, 4, 1, kOut>(p, kAll, st, what);
+  if (int rc = launch_tiles<256, 256, 4, 2, kOut>(p, kWhole, st, what)) return rc;
+  return launch_tiles<64, 128, 4, 1, kOut>(p, kLeft, st, what);
 }
 
 }  // namespace

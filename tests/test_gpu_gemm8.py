@@ -15,9 +15,10 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
-@pytest.fixture(params=[0, 1, 2], ids=["by_rule", "k_over_wavefronts", "tiles"], autouse=True)
+@pytest.fixture(params=[0, 1, 2, 3, 4, 5], ids=["by_rule", "k_over_wavefronts", "tiles", "tiles_of_128", "tiles_of_64", "tiles_and_rest"],
+                autouse=True)
 def form(request):
-    """Every test in the form that the library picks, and in either of the two."""
+    """Every test in the form that the library picks, and in each of them."""
     from ccfuser_amd import ops
     ops.set_option("fp8_form", request.param)
     yield request.param
