@@ -110,8 +110,9 @@ __device__ __forceinline__ Tile find_tile(const Gemm8Args &p, int pid, int grid,
 // in front of its last columns, whose fragment is in registers by then: behind it this step's place is free for the loads
 // of the step after the next, and the next step's rows are read between the last products, each into the registers that a
 // product has just let go.  So the matrix cores run through the steps, and a load has a whole step to land.
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int NS>
 struct TileShape {
+  static constexpr int kPlaces = NS;
   static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
   static constexpr int TT = BM / WM / 16, CT = BN / WN / 16;       // 16 x 16 products of a wavefront: rows, columns
   static constexpr int kRowsBytes = (BM + BN) * kScaleBlock;       // a place: codes, then scales of rows, then of columns
@@ -246,15 +247,32 @@ __device__ __forceinline__ void tile_sources(const Gemm8Args &p, const Tile &til
   }
 }
 
-// Persistent: a workgroup per CU runs tiles one behind the other, and the steps of all of them are one stream: the next
+// On to the step behind `next`'s next_kb, which is loaded; e < 0: there is none.
+template <class S, int BM, int BN>
+__device__ __forceinline__ void advance(const Gemm8Args &p, const TileMap<BM> &map, int end, int slots, int wave, int lane, int chunk,
+                                        int KB, int NB, Tile &next, int &next_kb, int &t_next, int &ahead,
+                                        uint32_t (&src)[S::kLoads], uint32_t &scale_src) {
+  ++ahead;
+  if (++next_kb < KB) return;
+  next_kb = 0;
+  t_next += slots;
+  if (t_next < end) {
+    next = map.find(t_next);
+    tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
+  } else {
+    next.e = -1;
+  }
+}
+
+// Persistent: a workgroup per CU (or two, of small tiles) runs tiles one behind the other, and the steps of all of them are one stream: the next
 // tile's first loads are on their way while this one's last products and its epilogue run.
-template <int BM, int BN, int WM, int WN, int kOut>
+template <int BM, int BN, int WM, int WN, int NS, int kOut>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
-  using S = TileShape<BM, BN, WM, WN>;
+  using S = TileShape<BM, BN, WM, WN, NS>;
   using Out = std::conditional_t<kOut == kGemm8Bf16, bf16_t, half_t>;
-  extern __shared__ __attribute__((aligned(1024))) char s_tile[];          // two places, then the tile map
-  int *s_map = reinterpret_cast<int *>(s_tile + 2 * S::kStage);
+  extern __shared__ __attribute__((aligned(1024))) char s_tile[];          // the places, then the tile map
+  int *s_map = reinterpret_cast<int *>(s_tile + NS * S::kStage);
   TileMap<BM>::build(p, part, s_map, s_map + p.E + 1);
   __syncthreads();
   const TileMap<BM> map{s_map, s_map + p.E + 1, p.E, n_tiles};
@@ -276,8 +294,8 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
   const float *scale_base = p.b_scale;
   if (scales_of_rows) scale_base = p.a_scale;
   // the step whose loads are issued next: tile `next` (e < 0: there is none), block next_kb
+  int t_now = t_next, next_kb = 0, ahead = 0;        // ahead: steps loaded beyond the one that is computed
   Tile next = map.find(t_next);
-  int next_kb = 0;
   tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
   const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)s_tile));
   // its loads in four parts (a wavefront that issues all at once waits for the queue and its products with it)
@@ -318,8 +336,13 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
     return join(*reinterpret_cast<const int4v *>(place + at + i * 16 * kScaleBlock),
                 *reinterpret_cast<const int4v *>(place + (at ^ 64) + i * 16 * kScaleBlock));
   };
-  float4v acc[S::CT][S::TT], product[S::TT];
-  int8v x[S::TT], w[2];
+  // Fragments of columns are read kRing - 1 ahead of their products, and a product's result is scaled three products later.
+  // With four rows' fragments to a column's one that is ahead enough; with fewer a column's products do not cover an LDS read,
+  // and three columns' do.
+  constexpr int kRing = S::TT >= 4 ? 2 : 4, kLate = 3, Q = S::CT * S::TT;
+  static_assert(S::CT % kRing == 0 && Q % (kLate + 1) == 0 && S::CT - kRing >= 4, "rings turn whole times in a step");
+  float4v acc[S::CT][S::TT], product[kLate + 1];
+  int8v x[S::TT], w[kRing], x_next[S::TT];
   float sa[S::TT], sb, s[S::TT];                     // scales as read for the coming step; of the step whose results are scaled
   auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -327,11 +350,16 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
 #pragma unroll
       for (int t = 0; t < S::TT; ++t) acc[c][t] = float4v{0, 0, 0, 0};
 #pragma unroll
-    for (int t = 0; t < S::TT; ++t) product[t] = float4v{0, 0, 0, 0}, s[t] = 0.0f;
-  };
-  auto scaled = [&](int c, int t) __attribute__((always_inline)) {
+    for (int q = 0; q <= kLate; ++q) product[q] = float4v{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[c][t][i] = fmaf(product[t][i], s[t], acc[c][t][i]);
+    for (int t = 0; t < S::TT; ++t) s[t] = 0.0f;
+  };
+  auto scaled = [&](int q) __attribute__((always_inline)) {          // of the step's Q products, in their order
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float4v &sum = acc[q / S::TT][q % S::TT];
+      sum[i] = fmaf(product[q % (kLate + 1)][i], s[q % S::TT], sum[i]);
+    }
   };
   // the sums of columns c exist here: without that the compiler puts all scalings of a step off behind its branch, and
   // keeps their inputs in registers that there are not
@@ -339,92 +367,111 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
 #pragma unroll
     for (int t = 0; t < S::TT; ++t) asm volatile("" : "+v"(acc[c][t]));
   };
-  auto meet = [&]() __attribute__((always_inline)) {                                  // all loads have landed, all LDS reads are done
-    __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
+  // the coming step's loads have landed (those of the ahead - 1 steps behind it may be on their way), all LDS reads are done
+  const bool more_loads = scales_of_rows || scales_of_columns;
+  auto meet = [&]() __attribute__((always_inline)) {
+    auto wait = [](auto N) __attribute__((always_inline)) {
+      constexpr int n = decltype(N)::value;
+      static_assert(n < 64, "vmcnt has six bits");
+      __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | (n >> 4) << 14);      // vmcnt(n) lgkmcnt(0)
+    };
+    if (NS == 2 || ahead <= 1) wait(std::integral_constant<int, 0>{});
+    else in_turn(std::make_integer_sequence<int, NS - 2>{}, [&](auto I) __attribute__((always_inline)) {
+      constexpr int behind = decltype(I)::value + 1;
+      if (ahead != behind + 1) return;
+      if (more_loads) wait(std::integral_constant<int, behind * (S::kLoads + 1)>{});
+      else wait(std::integral_constant<int, behind * S::kLoads>{});
+    });
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
 
   Tile tile = next;
-  in_turn(std::make_integer_sequence<int, kParts>{}, [&](auto I) __attribute__((always_inline)) { load_part(0, I); });
-  ++next_kb;                                         // (K has two blocks at least)
-  meet();
-  if (next.e >= 0) load_part(1, kFirst);
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (next.e >= 0) {
+      in_turn(std::make_integer_sequence<int, kParts>{}, [&](auto I) __attribute__((always_inline)) { load_part(i, I); });
+      advance<S, BM, BN>(p, map, end, slots, wave, lane, chunk, KB, NB, next, next_kb, t_next, ahead, src, scale_src);
+    }
+  meet();                                            // (ahead counts the step that comes)
+  --ahead;
+  if (next.e >= 0) load_part(NS - 1, kFirst);
   sb = *reinterpret_cast<const float *>(s_tile + sb_at);
 #pragma unroll
   for (int t = 0; t < S::TT; ++t) {
     x[t] = fragment(s_tile, x_at, t);
     sa[t] = *reinterpret_cast<const float *>(s_tile + sa_at + 64 * t);
   }
-  w[0] = fragment(s_tile, w_at, 0);
+#pragma unroll
+  for (int c = 0; c < kRing - 1; ++c) w[c] = fragment(s_tile, w_at, c);
   clear();
 
   int place = 0, kb = 0;
   while (true) {
     const char *now = s_tile + place * S::kStage;
-    // a product's result is scaled three products later
-    constexpr int last = S::CT - 1;
-    in_turn(std::make_integer_sequence<int, S::CT - 1>{}, [&](auto C) __attribute__((always_inline)) {
-      constexpr int c = decltype(C)::value, c_before = c ? c - 1 : last;           // (the step before's last columns)
-      w[(c + 1) & 1] = fragment(now, w_at, c + 1);
+    const int coming = place + 1 < NS ? place + 1 : 0;
+    const char *next_place = s_tile + coming * S::kStage;            // behind the last step: read for nothing
+    in_turn(std::make_integer_sequence<int, S::CT>{}, [&](auto C) __attribute__((always_inline)) {
+      constexpr int c = decltype(C)::value, c_ahead = c + kRing - 1;
+      constexpr bool at_meet = c == S::CT - kRing + 1, rows_here = S::TT >= 4 && c == S::CT - 1;
+      if constexpr (at_meet) {
+        meet();                                      // the next step's loads have landed, this one's place is read
+        if (next.e >= 0) load_part(place, kFirst);
+        --ahead;
+        if constexpr (S::TT < 4) {
 #pragma unroll
-      for (int t = 0; t < S::TT - 1; ++t) {
-        product[t] = mfma8(w[c & 1], x[t]);
-        scaled(c_before, t + 1);
-      }
-      if constexpr (c == 0) {
-#pragma unroll
-        for (int t = 0; t < S::TT; ++t) s[t] = sa[t] * sb;
-      }
-      product[S::TT - 1] = mfma8(w[c & 1], x[S::TT - 1]);
-      scaled(c, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-      for (int t = 0; t < S::TT; ++t) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-      }
-      settled(c_before);
-      __builtin_amdgcn_sched_barrier(0);
-      if (next.e >= 0) {
-        if constexpr (c < kParts - 1) load_part(place ^ 1, std::integral_constant<int, c + 1>{});
-        if constexpr (c == kParts - 1) {
-          if (++next_kb == KB) {
-            next_kb = 0;
-            t_next += slots;
-            if (t_next < end) {
-              next = map.find(t_next);
-              tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
-            } else {
-              next.e = -1;
-            }
+          for (int t = 0; t < S::TT; ++t) {
+            x_next[t] = fragment(next_place, x_at, t);
+            sa[t] = *reinterpret_cast<const float *>(next_place + sa_at + 64 * t);
           }
+          sb = *reinterpret_cast<const float *>(next_place + sb_at);
         }
       }
-    });
-    meet();                                          // the next step's loads have landed, this one's place is read
-    if (next.e >= 0) load_part(place, kFirst);
-    const char *ahead = s_tile + (place ^ 1) * S::kStage;            // behind the last step: read for nothing
+      if constexpr (!rows_here) w[c_ahead % kRing] = fragment(c_ahead < S::CT ? now : next_place, w_at, c_ahead % S::CT);
 #pragma unroll
-    for (int t = 0; t < S::TT; ++t) {
-      product[t] = mfma8(w[last & 1], x[t]);
-      if (t + 1 < S::TT) scaled(last - 1, t + 1);
-      else scaled(last, 0);
-      x[t] = fragment(ahead, x_at, t);
-      sa[t] = *reinterpret_cast<const float *>(ahead + sa_at + 64 * t);
+      for (int t = 0; t < S::TT; ++t) {
+        const int q = c * S::TT + t;
+        if (q == kLate) {
+#pragma unroll
+          for (int i = 0; i < S::TT; ++i) s[i] = sa[i] * sb;
+        }
+        product[q % (kLate + 1)] = mfma8(w[c % kRing], x[t]);
+        scaled((q + Q - kLate) % Q);
+        if constexpr (rows_here) {
+          x[t] = fragment(next_place, x_at, t);
+          sa[t] = *reinterpret_cast<const float *>(next_place + sa_at + 64 * t);
+        }
+      }
+      if constexpr (rows_here) {
+        w[0] = fragment(next_place, w_at, 0);
+        sb = *reinterpret_cast<const float *>(next_place + sb_at);
+      } else if constexpr (S::TT >= 4) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+        for (int t = 0; t < S::TT; ++t) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        }
+      }
+      settled(((Q + (c + 1) * S::TT - kLate) / S::TT + S::CT - 1) % S::CT);
+      __builtin_amdgcn_sched_barrier(0);
+      if (next.e >= 0) {
+        if constexpr (c < kParts - 1) load_part(place ? place - 1 : NS - 1, std::integral_constant<int, c + 1>{});
+        if constexpr (c == kParts - 1) advance<S, BM, BN>(p, map, end, slots, wave, lane, chunk, KB, NB, next, next_kb, t_next, ahead, src, scale_src);
+      }
+    });
+    if constexpr (S::TT < 4) {
+#pragma unroll
+      for (int t = 0; t < S::TT; ++t) x[t] = x_next[t];
     }
-    w[0] = fragment(ahead, w_at, 0);
-    sb = *reinterpret_cast<const float *>(ahead + sb_at);
-    settled(last - 1);
-    __builtin_amdgcn_sched_barrier(0);
-    place ^= 1;
+    place = coming;
     if (++kb < KB) continue;
 
     // the tile's end.  A lane holds one row and, in every product, four consecutive columns; of four products' columns it
     // stores 16 consecutive ones, which it gets from the lanes that hold the same row
 #pragma unroll
-    for (int t = 1; t < S::TT; ++t) scaled(last, t);
+    for (int q = Q - kLate; q < Q; ++q) scaled(q);
     const int rows = tile.rows < BM ? tile.rows : BM, n0 = tile.n * BN;
     const Out *bias = p.bias ? static_cast<const Out *>(p.bias) + static_cast<size_t>(tile.e) * p.N : nullptr;
     const int col0 = n0 + wn * (BN / WN), nb = block_of(col0);       // a wavefront's columns share a scale
@@ -493,8 +540,9 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
         }
       }
     }
-    if (next.e < 0) return;
-    tile = next;                                     // whose second step is loaded next (K has two blocks at least)
+    t_now += slots;
+    if (t_now >= end) return;
+    tile = map.find(t_now);
     kb = 0;
     clear();
   }
@@ -687,11 +735,11 @@ int compute_units() {
   return cached;
 }
 
-template <int BM, int BN, int WM, int WN, int kOut>
+template <int BM, int BN, int WM, int WN, int NS, int kOut>
 int launch_tiles(const Gemm8Args &p, int part, hipStream_t st, const char *what) {
-  using S = TileShape<BM, BN, WM, WN>;
-  auto kernel = gemm8_tile_kernel<BM, BN, WM, WN, kOut>;
-  const size_t lds = 2 * S::kStage + 4 * (3 * p.E + 1);
+  using S = TileShape<BM, BN, WM, WN, NS>;
+  auto kernel = gemm8_tile_kernel<BM, BN, WM, WN, NS, kOut>;
+  const size_t lds = NS * S::kStage + 4 * (3 * p.E + 1);
   const int cus = compute_units(), n_tiles = (p.N + BN - 1) / BN;
   CCF_REQUIRE(cus > 0, CCF_ERR_HIP, "%s: no device", what);
   if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), lds, what)) return rc;
@@ -719,20 +767,25 @@ int gemm8_out(const Gemm8Args &p, hipStream_t st, const char *what) {
   const int rows = (p.max_rows + owners - 1) / owners;         // of an expert, loads being even
   // (the 8-bit output wants all 128 columns of a scale in one workgroup)
   constexpr int CS = kOut == kGemm8Gelu8 ? 2 : 1;
-  const bool can_tile = p.K > kScaleBlock;                     // two steps at least
   int form = g_fp8_form;
   const long long large = static_cast<long long>(p.max_rows / 256 + owners) * ((p.N + 255) / 256);
-  if (form == 0) form = !can_tile || rows <= 32 ? 1 : (rows > 128 && large >= 256 ? 2 : (rows > 64 ? 3 : 4));
-  if (!can_tile) form = 1;
+  if (form == 0) form = rows <= 32 ? 1 : (rows > 128 && large >= 256 ? 2 : (rows > 64 ? 3 : 4));
   if (form == 1) {
     if (rows <= 16) return launch_split<1, 4, CS, kOut>(p, st, what);
     return launch_split<2, 4, CS, kOut>(p, st, what);
   }
-  if (form == 2) return launch_tiles<256, 256, 4, 2, kOut>(p, kAll, st, what);
-  if (form == 3) return launch_tiles<128, 128, 4, 1, kOut>(p, kAll, st, what);
-  if (form == 4) return launch_tiles<64, 128, 4, 1, kOut>(p, kAll, st, what);
-  if (int rc = launch_tiles<256, 256, 4, 2, kOut>(p, kWhole, st, what)) return rc;
-  return launch_tiles<64, 128, 4, 1, kOut>(p, kLeft, st, what);
+  if (form == 2) return launch_tiles<256, 256, 4, 2, 2, kOut>(p, kAll, st, what);
+  if (form == 3) return launch_tiles<128, 128, 4, 1, 2, kOut>(p, kAll, st, what);
+  if (form == 4) return launch_tiles<64, 128, 4, 1, 3, kOut>(p, kAll, st, what);
+#ifdef SWEEP
+  if (form == 6) return launch_tiles<128, 128, 4, 1, 4, kOut>(p, kAll, st, what);
+  if (form == 7) return launch_tiles<128, 128, 8, 1, 4, kOut>(p, kAll, st, what);
+  if (form == 8) return launch_tiles<64, 128, 4, 1, 6, kOut>(p, kAll, st, what);
+  if (form == 9) return launch_tiles<64, 128, 4, 1, 2, kOut>(p, kAll, st, what);
+  if (form == 10) return launch_tiles<128, 256, 4, 2, 3, kOut>(p, kAll, st, what);
+#endif
+  if (int rc = launch_tiles<256, 256, 4, 2, 2, kOut>(p, kWhole, st, what)) return rc;
+  return launch_tiles<64, 128, 4, 1, 3, kOut>(p, kLeft, st, what);
 }
 
 }  // namespace

@@ -98,7 +98,7 @@ const char *ccf_last_error(void);
  *                     ccf_moe_forward the gate kernel leaves such a table when it fits (and top_k is a power
  *                     of two), and the routing stage is then one launch.  0 = always histogram, scan, pos
  *   "fp8_form"        0 (default): products in 8 bits run as 256-row tiles through LDS or, for few rows or few tiles, with K
- *                     cut over the wavefronts of a workgroup; 1 = the second always, 2 = the first (K of 256 and more)
+ *                     cut over the wavefronts of a workgroup; see gemm8.hip
  *   "gate_slots"      0, 1, 2 or 4: parts of K a gate wavefront works on at a time, which divides the tokens
  *                     of a workgroup by the same number (0 = chosen by the token count)
  *   "dgrad_transpose" 0/1: the backward's input-gradient GEMM runs on a transposed copy of the
