@@ -8,9 +8,11 @@
 // instruction's own scales are powers of two per 32 elements; weights come with scales of any value.)  A lane's 32
 // bytes are the same ones of either operand, in whatever order of K: all that a product needs.
 //
-// Two kernels.  gemm8_tile_kernel: tiles through LDS, for many rows: bound by the matrix cores.  gemm8_split_kernel: a
-// workgroup's wavefronts cut K among them and read straight from memory, for few rows or few tiles: bound by the weights'
-// bytes or by a chain of loads.
+// Two kernels.  gemm8_tile_kernel: tiles of 256, 128 or 64 rows through LDS.  It is bound by the instructions that a SIMD
+// issues: at 4096 rows, 4096 -> 14336, 252 us (1.9 PFLOP/s) and 225 with the loads of operands left out; the four fused
+// multiply-adds per product, which any fp32 scale needs, are most of them.  gemm8_split_kernel: a workgroup's wavefronts cut K
+// among them and read straight from memory, for few rows or few tiles: bound by the weights' bytes or by a chain of loads
+// (1 row, 4096 -> 14336: 14.8 us, 4.0 TB/s).
 #include "gemm8.h"
 #include "gelu.h"
 
@@ -18,7 +20,7 @@
 #include <utility>
 
 namespace ccf {
-int g_fp8_form = 0;          // 0: by the rule of gemm8_out; 1: K cut over the wavefronts always; 2: tiles through LDS always
+int g_fp8_form = 0;          // 0: by form_of's rule, else a Form for every call
 namespace {
 
 __device__ const int4v kZeros16 = {0, 0, 0, 0};              // what lanes behind the end of K read
@@ -101,7 +103,7 @@ __device__ __forceinline__ Tile find_tile(const Gemm8Args &p, int pid, int grid,
 // ------------------------------------------------------------------ tiles through LDS
 //
 // BM rows x BN columns, WM x WN wavefronts; a K step is a block of 128, staged by direct loads into one of two LDS places
-// while the other is multiplied.  16-byte chunks of a row lie at chunk ^ (row % 8), which the loads' global addresses apply,
+// while the other is multiplied (of the small tile three, so that a load has two steps to land).  16-byte chunks of a row lie at chunk ^ (row % 8), which the loads' global addresses apply,
 // and a lane's two chunks are g and g + 4 (g = lane / 16): a read then takes 5 cycles of a wavefront (256 bytes each),
 // with 2 g and 2 g + 1 9, unswizzled 17.  The scales of a step come the same way, a
 // lane per row, and lie by row.
@@ -251,21 +253,26 @@ __device__ __forceinline__ void tile_sources(const Gemm8Args &p, const Tile &til
 template <class S, int BM, int BN>
 __device__ __forceinline__ void advance(const Gemm8Args &p, const TileMap<BM> &map, int end, int slots, int wave, int lane, int chunk,
                                         int KB, int NB, Tile &next, int &next_kb, int &t_next, int &ahead,
+                                        const uint8_t *&a, const uint8_t *&b,
                                         uint32_t (&src)[S::kLoads], uint32_t &scale_src) {
   ++ahead;
+  a += kScaleBlock;
+  b += kScaleBlock;
   if (++next_kb < KB) return;
   next_kb = 0;
   t_next += slots;
   if (t_next < end) {
     next = map.find(t_next);
+    a = p.a;
+    b = p.b + static_cast<size_t>(next.e) * p.N * p.K;
     tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
   } else {
     next.e = -1;
   }
 }
 
-// Persistent: a workgroup per CU (or two, of small tiles) runs tiles one behind the other, and the steps of all of them are one stream: the next
-// tile's first loads are on their way while this one's last products and its epilogue run.
+// Persistent: a workgroup per CU (or two, of small tiles) runs tiles one behind the other, and the steps of all of them are
+// one stream: the next tile's first loads are on their way while this one's last products and its epilogue run.
 template <int BM, int BN, int WM, int WN, int NS, int kOut>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
@@ -296,16 +303,16 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
   // the step whose loads are issued next: tile `next` (e < 0: there is none), block next_kb
   int t_now = t_next, next_kb = 0, ahead = 0;        // ahead: steps loaded beyond the one that is computed
   Tile next = map.find(t_next);
+  const uint8_t *a = p.a, *b = p.b + static_cast<size_t>(next.e) * p.N * p.K;
   tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
   const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)s_tile));
-  // its loads in four parts (a wavefront that issues all at once waits for the queue and its products with it)
-  constexpr int kParts = 4;
+  // Its loads in four parts: a wavefront that issues all at once waits for the queue, and its products with it.  A wavefront
+  // of few products, which are done before its instructions are issued, has fewer of those with all loads in one.
+  constexpr int kParts = S::TT >= 4 ? 4 : 1;
   constexpr std::integral_constant<int, 0> kFirst{};
   auto load_part = [&](int place, auto PART) __attribute__((always_inline)) {
     constexpr int quarter = decltype(PART)::value;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds + place * S::kStage + wave * 1024);
-    const uint8_t *a = p.a + next_kb * kScaleBlock;
-    const uint8_t *b = p.b + static_cast<size_t>(next.e) * p.N * p.K + next_kb * kScaleBlock;
     constexpr int lo = quarter * S::kLoads / kParts, hi = (quarter + 1) * S::kLoads / kParts;
     if (tail && next_kb == KB - 1) {
       // chunks behind the end of K: zeros for the rows, and for the columns the block's first chunk again (what is no
@@ -392,11 +399,19 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
   for (int i = 0; i < NS - 1; ++i)
     if (next.e >= 0) {
       in_turn(std::make_integer_sequence<int, kParts>{}, [&](auto I) __attribute__((always_inline)) { load_part(i, I); });
-      advance<S, BM, BN>(p, map, end, slots, wave, lane, chunk, KB, NB, next, next_kb, t_next, ahead, src, scale_src);
+      advance<S, BM, BN>(p, map, end, slots, wave, lane, chunk, KB, NB, next, next_kb, t_next, ahead, a, b, src, scale_src);
     }
-  meet();                                            // (ahead counts the step that comes)
-  --ahead;
-  if (next.e >= 0) load_part(NS - 1, kFirst);
+  auto on = [&]() __attribute__((always_inline)) {
+    advance<S, BM, BN>(p, map, end, slots, wave, lane, chunk, KB, NB, next, next_kb, t_next, ahead, a, b, src, scale_src);
+  };
+  auto begin_load = [&](int place) __attribute__((always_inline)) {
+    --ahead;                                         // (which counted the step that comes)
+    if (next.e < 0) return;
+    load_part(place, kFirst);
+    if constexpr (kParts == 1) on();
+  };
+  meet();
+  begin_load(NS - 1);
   sb = *reinterpret_cast<const float *>(s_tile + sb_at);
 #pragma unroll
   for (int t = 0; t < S::TT; ++t) {
@@ -417,8 +432,7 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
       constexpr bool at_meet = c == S::CT - kRing + 1, rows_here = S::TT >= 4 && c == S::CT - 1;
       if constexpr (at_meet) {
         meet();                                      // the next step's loads have landed, this one's place is read
-        if (next.e >= 0) load_part(place, kFirst);
-        --ahead;
+        begin_load(place);
         if constexpr (S::TT < 4) {
 #pragma unroll
           for (int t = 0; t < S::TT; ++t) {
@@ -456,9 +470,11 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
       }
       settled(((Q + (c + 1) * S::TT - kLate) / S::TT + S::CT - 1) % S::CT);
       __builtin_amdgcn_sched_barrier(0);
-      if (next.e >= 0) {
-        if constexpr (c < kParts - 1) load_part(place ? place - 1 : NS - 1, std::integral_constant<int, c + 1>{});
-        if constexpr (c == kParts - 1) advance<S, BM, BN>(p, map, end, slots, wave, lane, chunk, KB, NB, next, next_kb, t_next, ahead, src, scale_src);
+      if constexpr (kParts > 1 && c < kParts) {
+        if (next.e >= 0) {
+          if constexpr (c < kParts - 1) load_part(place ? place - 1 : NS - 1, std::integral_constant<int, c + 1>{});
+          else on();
+        }
       }
     });
     if constexpr (S::TT < 4) {
@@ -761,29 +777,44 @@ int launch_split(const Gemm8Args &p, hipStream_t st, const char *what) {
   return check_launch(what);
 }
 
+// The form by sizes; the experts' row counts are on the device, so their loads are taken as even, and a quarter more.  The
+// limits are where measured times cross (us, K -> N, rows of an expert; weights cycled through a graph's replays):
+//   K over wavefronts, for at most 32 rows, where one round of workgroups holds them and K is long: 4096 -> 14336, 1 row
+//   14.8 and tiles of 64 21.7; 8192 -> 2048 of 8 experts, 8 rows 26 and 40; but 768 -> 2048 7.8 and 6.9, and in two rounds
+//   (14336 -> 4096 of 8, 2 rows) 86 and 77.
+//   Tiles of 64, while there are few tiles: 4096 -> 1024, 512 rows 22, of 128 28, of 256 51; 4096 -> 14336, 333 rows 47, 41, 56.
+//   Tiles of 256 with the rest as a launch of its own, where the whole tiles alone fill the chip: 4096 -> 14336 of 8, 512
+//   rows 364, all in tiles of 256 394, of 128 397; but 4096 -> 1024, 4096 rows 56, 54, 32.
+//   Tiles of 256, where tiles of 128 go over a round: 4096 -> 14336, 700 rows 60, of 128 68; 512 rows 56 and 45.
+enum Form { kSplit = 1, kTiles256, kTiles128, kTiles64, kTilesAndRest };
+Form form_of(const Gemm8Args &p) {
+  constexpr long long kCus = 256;
+  const bool grouped = p.offsets != nullptr;
+  const long long owners = grouped ? (p.E < p.max_rows ? p.E : p.max_rows) : 1;
+  const long long rows = (p.max_rows + owners - 1) / owners, likely = grouped ? rows + rows / 4 : rows;
+  auto tiles = [&](int bm, int bn) { return owners * ((likely + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+  if (p.K >= 2048 && (grouped ? 2 * rows : rows) <= 32 && owners * ((p.N + 63) / 64) <= kCus) return kSplit;
+  if (owners * (rows / kWholeRows) * ((p.N + 255) / 256) >= kCus) return kTilesAndRest;
+  if (likely <= 64 || tiles(64, 128) <= 448) return kTiles64;
+  if (likely > 128 && tiles(128, 128) >= 640) return kTiles256;
+  return kTiles128;
+}
+
 template <int kOut>
 int gemm8_out(const Gemm8Args &p, hipStream_t st, const char *what) {
-  const int owners = p.offsets ? (p.E < p.max_rows ? p.E : p.max_rows) : 1;
-  const int rows = (p.max_rows + owners - 1) / owners;         // of an expert, loads being even
   // (the 8-bit output wants all 128 columns of a scale in one workgroup)
   constexpr int CS = kOut == kGemm8Gelu8 ? 2 : 1;
-  int form = g_fp8_form;
-  const long long large = static_cast<long long>(p.max_rows / 256 + owners) * ((p.N + 255) / 256);
-  if (form == 0) form = rows <= 32 ? 1 : (rows > 128 && large >= 256 ? 2 : (rows > 64 ? 3 : 4));
-  if (form == 1) {
-    if (rows <= 16) return launch_split<1, 4, CS, kOut>(p, st, what);
-    return launch_split<2, 4, CS, kOut>(p, st, what);
+  switch (g_fp8_form ? static_cast<Form>(g_fp8_form) : form_of(p)) {
+    case kSplit: {
+      // 16 rows at a time, or 32 where an expert probably has more
+      const int rows = p.offsets ? 2 * ((p.max_rows + p.E - 1) / p.E) : p.max_rows;
+      return rows <= 16 ? launch_split<1, 4, CS, kOut>(p, st, what) : launch_split<2, 4, CS, kOut>(p, st, what);
+    }
+    case kTiles256: return launch_tiles<256, 256, 4, 2, 2, kOut>(p, kAll, st, what);
+    case kTiles128: return launch_tiles<128, 128, 4, 1, 2, kOut>(p, kAll, st, what);
+    case kTiles64: return launch_tiles<64, 128, 4, 1, 3, kOut>(p, kAll, st, what);
+    default: break;
   }
-  if (form == 2) return launch_tiles<256, 256, 4, 2, 2, kOut>(p, kAll, st, what);
-  if (form == 3) return launch_tiles<128, 128, 4, 1, 2, kOut>(p, kAll, st, what);
-  if (form == 4) return launch_tiles<64, 128, 4, 1, 3, kOut>(p, kAll, st, what);
-#ifdef SWEEP
-  if (form == 6) return launch_tiles<128, 128, 4, 1, 4, kOut>(p, kAll, st, what);
-  if (form == 7) return launch_tiles<128, 128, 8, 1, 4, kOut>(p, kAll, st, what);
-  if (form == 8) return launch_tiles<64, 128, 4, 1, 6, kOut>(p, kAll, st, what);
-  if (form == 9) return launch_tiles<64, 128, 4, 1, 2, kOut>(p, kAll, st, what);
-  if (form == 10) return launch_tiles<128, 256, 4, 2, 3, kOut>(p, kAll, st, what);
-#endif
   if (int rc = launch_tiles<256, 256, 4, 2, 2, kOut>(p, kWhole, st, what)) return rc;
   return launch_tiles<64, 128, 4, 1, 3, kOut>(p, kLeft, st, what);
 }
@@ -804,6 +835,11 @@ int check_product(const Gemm8Args &p, const char *what) {
   CCF_REQUIRE(p.E <= 1024, CCF_ERR_SHAPE, "%s: num_expert=%d beyond 1024", what, p.E);
   CCF_REQUIRE(p.K % 16 == 0 && p.N % 8 == 0, CCF_ERR_SHAPE, "%s: contraction of %d and %d columns: multiples of 16 and 8 are needed",
               what, p.K, p.N);
+  // the tile kernel counts 16-byte chunks of the rows, and bytes of an expert's weights, in 32 bits
+  CCF_REQUIRE(p.max_rows < (1 << 30) && static_cast<long long>(p.max_rows) * (p.K / 16) < (1ll << 32) &&
+                  static_cast<long long>(p.N) * p.K < (1ll << 32), CCF_ERR_SHAPE,
+              "%s: %d rows of %d and %d columns: rows times contraction reaches 2^36 or columns times contraction 2^32", what,
+              p.max_rows, p.K, p.N);
   if (p.max_rows == 0) return CCF_OK;
   CCF_REQUIRE(p.a && p.a_scale && p.b && p.b_scale && (p.c || (p.codes && p.scales)), CCF_ERR_ARG, "%s: null pointer", what);
   CCF_REQUIRE(aligned16(p.a) && aligned16(p.b) && aligned16(p.c) && aligned16(p.codes) && aligned16(p.bias), CCF_ERR_ARG,
