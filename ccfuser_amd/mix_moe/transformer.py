@@ -7,6 +7,7 @@ from .. import ops
 from .gates import NaiveGate
 from .layers import MixMOE
 from .linear import FMoELinear, MixMOEFusedFFN, MixMOEInstance, MixMOELinear1, MixMOELinear2, _pair
+from .norm import RMSNorm
 
 _COMPAT_KEYS = ("expert_ids", "local_expert_id_indexs", "ranks", "lens", "start_addrs",
                 "remote_block_num", "total_block_num", "expert_block_ids", "expert_block_id_idxs")
@@ -205,12 +206,19 @@ class MixMOETransformerMLP(MixMOE):
     through ``process_data`` and ``MixMOE.forward`` like the reference.  When a
     gradient is wanted (grad mode on and the input or a parameter requires it)
     the staged path runs, whose stages carry their backward.
+
+    Not in the reference either: ``pre_norm=True`` puts an ``RMSNorm`` (``norm``)
+    in front of the gate and the experts; ``few_tokens=n`` hands fused calls of at
+    most n tokens (32 at most, no capacity factor) to ``ops.moe_forward_few``;
+    ``quantize_experts()`` lets fused calls run on experts in 8 bits.
     """
 
     def __init__(self, gate_type, experts, model_dim: int, expert_rank, world_size,
                  scan_expert_func=None, total_batch_size=4096, expert_dp_comm="none",
                  activation=torch.nn.GELU(), mix_moe=None, capacity_factor=None, fused=True,
-                 popular_expert_num=3, **kwargs):
+                 popular_expert_num=3, pre_norm=False, norm_eps=1e-5, few_tokens=0, **kwargs):
+        if not 0 <= few_tokens <= ops.FEW_TOKENS:
+            raise ValueError(f"few_tokens={few_tokens} outside 0..{ops.FEW_TOKENS}")
         super().__init__(num_expert=experts["num_local_expert"], d_model=model_dim,
                          ffn_hidden_size=experts["hidden_size"], expert=None, my_rank=expert_rank,
                          world_size=world_size, **kwargs)
@@ -224,6 +232,9 @@ class MixMOETransformerMLP(MixMOE):
         self.async_ = False
         self.capacity_factor = capacity_factor
         self.fused = fused
+        self.few_tokens = few_tokens
+        self.norm = RMSNorm(model_dim, norm_eps) if pre_norm else None
+        self._experts8 = None
         self.async_expert_assign = AsyncExpertAssignment(expert_rank, world_size, popular_expert_num,
                                                          experts["num_local_expert"], total_batch_size)
 
@@ -232,8 +243,38 @@ class MixMOETransformerMLP(MixMOE):
             return -1
         return int(-(-self.capacity_factor * tokens * self.top_k // self.num_expert))
 
+    def quantize_experts(self, on=True):
+        """Lays the experts' weights out in 8 bits (e4m3, a scale for each 128 x 128 block) beside the stored ones; from then on
+        a fused call without gradients multiplies those.  Staged, asynchronous and differentiable calls keep to the stored
+        weights.  The layout is of this moment: once the stored weights change, calls are refused until it is made anew,
+        or dropped with ``on=False``."""
+        self._experts8 = None
+        if not on:
+            return self
+        if not (self.fused and self.experts._gelu_is_fusable()):
+            raise ValueError("quantize_experts: only fused layers with the erf GELU run on experts in 8 bits")
+        up, down = self.experts.htoh4.weight, self.experts.h4toh.weight
+        E = self.num_expert
+        self._experts8 = (*ops.quantize_weight(up.detach()[:E].contiguous()), *ops.quantize_weight(down.detach()[:E].contiguous()),
+                          (up._version, down._version))
+        return self
+
+    def _forward_fp8(self, inp):
+        w1, s1, w2, s2, versions = self._experts8
+        lin, up, down = self.gate.gate, self.experts.htoh4, self.experts.h4toh
+        if (up.weight._version, down.weight._version) != versions:
+            raise RuntimeError("expert weights have changed since quantize_experts()")
+        x_fp8 = None
+        if self.norm is not None:
+            n = ops.rms_norm(inp, self.norm.weight, self.norm.eps, want_fp8=True)
+            inp, x_fp8 = n.y, (n.codes, n.scale)
+        b1, b2 = (None if b is None else b.detach()[:self.num_expert] for b in (up.bias, down.bias))
+        return ops.moe_forward_fp8(inp, lin.weight, lin.bias, w1, s1, b1, w2, s2, b2, self.top_k, self._capacity(inp.shape[0]), x_fp8)
+
     def async_expert_assignment(self, attn_inp: torch.Tensor):
         inp = attn_inp.reshape(-1, self.d_model)
+        if self.norm is not None:
+            inp = self.norm(inp)
         self.async_expert_assign.capacity = self._capacity(inp.shape[0])
         self.async_expert_assign.add_task(self.gate, inp, self.num_expert, self.world_size)
         self.async_ = True
@@ -251,17 +292,26 @@ class MixMOETransformerMLP(MixMOE):
         if not inp.is_contiguous():
             inp = inp.contiguous()
         E = self.num_expert
+        fused = not self.async_ and self.fused and self.experts._gelu_is_fusable() and not (
+            torch.is_grad_enabled() and (inp.requires_grad or _any_requires_grad(self)))
+        if fused and self._experts8 is not None:
+            output = self._forward_fp8(inp)
+            return output if rows else output.reshape(original_shape)
+        if self.norm is not None:
+            inp = self.norm(inp)
         if self.async_:
             self.async_expert_assign.wait_for_completion()
             pos, gate_score, infos = self.async_expert_assign.result
             self.async_ = False
             output = super().forward(inp, pos, gate_score, infos)
-        elif self.fused and self.experts._gelu_is_fusable() and not (
-                torch.is_grad_enabled() and (inp.requires_grad or _any_requires_grad(self))):
+        elif fused:
             ex = self.experts
             lin, up, down = self.gate.gate, ex.htoh4, ex.h4toh
-            output = ops.moe_forward(inp, lin.weight, lin.bias, *_pair(up.weight, up.bias, E), *_pair(down.weight, down.bias, E),
-                                     self.top_k, self._capacity(inp.shape[0]), spare_experts=True)
+            weights = (lin.weight, lin.bias, *_pair(up.weight, up.bias, E), *_pair(down.weight, down.bias, E))
+            if inp.shape[0] <= self.few_tokens and self.capacity_factor is None:
+                output = ops.moe_forward_few(inp, *weights, self.top_k, spare_experts=True)
+            else:
+                output = ops.moe_forward(inp, *weights, self.top_k, self._capacity(inp.shape[0]), spare_experts=True)
         else:
             self.async_expert_assign.capacity = self._capacity(inp.shape[0])
             pos, gate_score, infos = self.async_expert_assign.process_data(

@@ -867,6 +867,8 @@ def _rows_fp8(x, name: str):
         return quantize_rows(x)
     codes, scale = x
     _check_fp8(codes, scale, name, False, 2)
+    if codes.numel() >= 1 << 36:                       # the products count a row's 16-byte chunks in 32 bits
+        raise ValueError(f"{name}: {tuple(codes.shape)} has 2^36 elements or more")
     return codes, scale
 
 

@@ -57,3 +57,69 @@ def test_no_cpu_path():
     for call in (lambda: ops.rms_norm(x, w), lambda: ops.quantize_rows(x), lambda: ops.quantize_weight(x), lambda: RMSNorm(64)(x)):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+def _linear(lib, x=FAKE, xs=FAKE, rows=2, k=64, w=FAKE, ws=FAKE, n=64, bias=None, dtype=0, y=FAKE):
+    return lib.ccf_linear_fp8(x, xs, rows, k, w, ws, n, bias, dtype, y, None)
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(rows=-1), 1), (dict(k=0), 1), (dict(n=0), 1), (dict(k=24), 2), (dict(n=12), 2), (dict(x=None), 1), (dict(xs=None), 1),
+    (dict(w=None), 1), (dict(ws=None), 1), (dict(y=None), 1), (dict(x=FAKE + 1), 1), (dict(w=FAKE + 8), 1), (dict(y=FAKE + 2), 1),
+    (dict(bias=FAKE + 2), 1), (dict(dtype=1), 5), (dict(dtype=9), 5), (dict(rows=1 << 30), 2), (dict(rows=1 << 24, k=1 << 16), 2),
+    (dict(k=1 << 17, n=1 << 15), 2)])
+def test_linear_refuses(lib, bad, code):
+    assert _linear(lib, **bad) == code
+    assert lib.ccf_last_error()
+
+
+def test_no_rows_are_no_call(lib):
+    assert _linear(lib, rows=0, x=None, xs=None, y=None) == 0
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(rows=-1), 1), (dict(E=0), 1), (dict(E=1025), 2), (dict(d=24), 2), (dict(f=12), 2), (dict(x=None), 1), (dict(off=None), 1),
+    (dict(w=None), 1), (dict(out=None), 1), (dict(b=FAKE + 2), 1)])
+def test_grouped_products_refuse(lib, bad, code):
+    a = dict(x=FAKE, xs=FAKE, src=None, off=FAKE, rows=4, E=2, d=64, f=64, w=FAKE, ws=FAKE, b=None, out=FAKE, out_s=FAKE)
+    a.update(bad)
+    assert lib.ccf_ffn1_fp8(a["x"], a["xs"], a["src"], a["off"], a["rows"], a["E"], a["d"], a["f"], a["w"], a["ws"], a["b"], a["out"],
+                            a["out_s"], None) == code
+    if "d" in bad or "f" in bad:                       # the other product contracts the other width
+        a["d"], a["f"] = a["f"], a["d"]
+    assert lib.ccf_ffn2_fp8(a["x"], a["xs"], a["src"], a["off"], a["rows"], a["E"], a["d"], a["f"], a["w"], a["ws"], a["b"], a["out"],
+                            None) == code
+
+
+LAYER = dict(T=4, d=64, f=64, E=4, k=2)
+
+
+def _layer(lib, **bad):
+    a = dict(x=FAKE, xc=None, xs=None, wg=FAKE, bg=None, w1=FAKE, s1=FAKE, b1=None, w2=FAKE, s2=FAKE, b2=None, cap=-1, out=FAKE, ws=FAKE,
+             nbytes=1 << 30, **LAYER)
+    a.update(bad)
+    return lib.ccf_moe_forward_fp8(a["x"], a["xc"], a["xs"], a["wg"], a["bg"], a["w1"], a["s1"], a["b1"], a["w2"], a["s2"], a["b2"], a["T"],
+                                   a["d"], a["f"], a["E"], a["k"], a["cap"], a["out"], None, None, a["ws"], a["nbytes"], None)
+
+
+def _few(lib, **bad):
+    a = dict(x=FAKE, wg=FAKE, bg=None, w1=FAKE, b1=None, w2=FAKE, b2=None, out=FAKE, ws=FAKE, nbytes=1 << 30, **LAYER)
+    a.update(bad)
+    return lib.ccf_moe_forward_few(a["x"], a["wg"], a["bg"], a["w1"], a["b1"], a["w2"], a["b2"], a["T"], a["d"], a["f"], a["E"], a["k"],
+                                   a["out"], None, None, a["ws"], a["nbytes"], None)
+
+
+@pytest.mark.parametrize("bad", [dict(T=-1), dict(d=72), dict(f=72), dict(E=0), dict(E=1025), dict(k=0), dict(k=5), dict(k=9, E=16),
+                                 dict(x=None), dict(wg=None), dict(w1=None), dict(w2=None), dict(out=None), dict(ws=None), dict(nbytes=8),
+                                 dict(x=FAKE + 2), dict(w1=FAKE + 8)], ids=str)
+def test_layers_refuse(lib, bad):
+    assert _layer(lib, **bad) not in (0, 4)
+    assert _few(lib, **bad) not in (0, 4)
+    assert lib.ccf_last_error()
+
+
+def test_layers_refuse_what_is_their_own(lib):
+    assert _few(lib, T=33) != 0
+    assert _layer(lib, s1=None) == 1 and _layer(lib, s2=None) == 1 and _layer(lib, xc=FAKE) == 1
+    for f in (lib.ccf_moe_few_workspace_bytes, lib.ccf_moe_fp8_workspace_bytes):
+        assert f(4, 64, 64, 4, 2) > 0
