@@ -13,10 +13,11 @@
 //   * the second kernel runs all chosen experts of its 16 columns into one sum, so nothing is left to combine.
 //
 // In 8 bits (e4m3, a scale per block of 128) rows of x are quantised where they are read, as ccf_quantize_rows does, and
-// the first kernel's workgroups have the 128 columns of a scale of h.  Wavefronts cut K among them and read straight from
-// memory, 16 rows of 128 consecutive bytes at a time, two steps ahead; their sums meet in LDS in a fixed order.
-// Workgroups start their sums at K places of their own, which go by the column: started together, they read the same bytes
-// of rows a power of two apart, and few of the memory's channels (XXX).
+// the first kernel's workgroups have the 128 columns of a scale of h.  Wavefronts cut K among them, each with a stream of
+// operands of its own; their sums meet in LDS in a fixed order.
+//
+// One token, widths 4096 and 14336, two experts: 16 bits 45 + 38 us, 5.3 and 6.2 TB/s (the gate is 5 to 8 us of the first),
+// 8 bits 31 + 22 us, 3.8 and 5.3 TB/s; 1 GiB copied by the framework 5.1.
 #include "few_layer.h"
 #include "gate_select.h"
 #include "gelu.h"
@@ -389,24 +390,19 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
     x_lane[j] = (t < T ? t : T - 1) * row_bytes + chunk * 16;
   }
 
-  // the item that is loaded next: the q-th of this wavefront's steps in unit u.  Its steps come in turn, from the one on that
-  // the unit's columns start at.
-  int u_next = blockIdx.x, q_next = 0, from_next = 0, slot_next = 0, ahead = 0;
+  // the item that is loaded next: the q-th of this wavefront's steps in unit u
+  int u_next = blockIdx.x, q_next = 0, slot_next = 0, ahead = 0;
   const uint8_t *w = nullptr;
   auto aim = [&]() __attribute__((always_inline)) {
     const int i = u_next / blocks, block = u_next - i * blocks;
     int c0 = block * BN + cs * 16;
     c0 = c0 < p.f ? c0 : p.f - 16;                 // (f is a multiple of 64) the second half of 128 columns: never stored
     const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
-    from_next = block % turns;
     w = static_cast<const uint8_t *>(p.w1) + (static_cast<size_t>(e) * p.f + c0) * row_bytes;
   };
-  auto step_of = [&](int from, int q) {
-    const int at = from + q, st = ks + (at < turns ? at : at - turns) * KS;
-    return st < steps ? st : steps - 1;
-  };
+  auto step_of = [&](int q) { return ks + q * KS < steps ? ks + q * KS : steps - 1; };
   auto load_item = [&]() __attribute__((always_inline)) {
-    const int st = step_of(from_next, q_next);
+    const int st = step_of(q_next);
     const uint8_t *base = w + st * 128, *base8 = base + static_cast<size_t>(8) * row_bytes;
     uint32_t at = ring_at + slot_next * S::kItem, lane_at = w_lane;
     // chunks behind the end of a row: its step's first one again, for codes that are zeros
@@ -435,14 +431,13 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
   constexpr int kPer = BN / 8;
   static_assert(16 * RB * kPer <= kThreads, "a thread has at most one piece of the epilogue");
   const int t_mine = threadIdx.x / kPer, c_mine = threadIdx.x % kPer * 8;
-  int u = blockIdx.x, q = 0, from = 0, i = 0, n0 = 0, slot = 255, place = 0;
+  int u = blockIdx.x, q = 0, i = 0, n0 = 0, slot = 255, place = 0;
   const float *sb = nullptr;
   half8 bias;
   float4v acc[RB];
   auto begin = [&]() __attribute__((always_inline)) {
     i = u / blocks;
     const int block = u - i * blocks, e = __builtin_amdgcn_readfirstlane(slots.act[i]);
-    from = block % turns;
     n0 = block * BN;
     if constexpr (kFp8) sb = p.s1 + (static_cast<size_t>(e) * FB + block) * KB;
     slot = t_mine < T && n0 + c_mine < p.f ? slots.of(i, t_mine) : 255;
@@ -506,7 +501,7 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
     else loads_but<0>();                           // the last items: none are loaded behind them
     const char *at = ring + place * S::kItem;
     place = place + 1 < S::kDepth ? place + 1 : 0;
-    const int st = step_of(from, q);
+    const int st = step_of(q);
     const int8v wf = fragment(at, r16, g);
     int8v xf[RB];
     float sx[RB];
@@ -609,8 +604,7 @@ few_layer_down_kernel(FewLayerArgs p) {
     w_lane[j] = r % CW * row_bytes + w_behind[j];
   }
   // the item that is loaded next: step `at` of chosen expert `i`, a token that did not choose it taking a row of one that did
-  const int from = count > 0 ? wave + blockIdx.x % count * kWaves : 0;
-  int i_next = 0, at_next = from, slot_next = 0, ahead = 0;
+  int i_next = 0, at_next = wave, slot_next = 0, ahead = 0;
   const uint8_t *w = nullptr;
   uint32_t h_lane[RB * NX], s_lane = 0;
   auto aim = [&]() __attribute__((always_inline)) {
@@ -628,7 +622,7 @@ few_layer_down_kernel(FewLayerArgs p) {
     if constexpr (kFp8) s_lane = row_of(lane % (16 * RB)) * KB;
   };
   auto load_item = [&]() __attribute__((always_inline)) {
-    if (at_next == from) aim();
+    if (at_next == wave) aim();
     const uint8_t *base = w + static_cast<size_t>(at_next) * (128 * KG), *h = static_cast<const uint8_t *>(p.h) + at_next * (128 * KG);
     const uint32_t at = ring_at + slot_next * S::kItem;
     const int left = row_bytes - at_next * (128 * KG);         // bytes of a row from this item on
@@ -663,13 +657,15 @@ few_layer_down_kernel(FewLayerArgs p) {
     ++ahead;
     slot_next = slot_next + 1 < S::kDepth ? slot_next + 1 : 0;
     at_next += kWaves;
-    if (at_next >= steps) at_next = wave;
-    if (at_next == from) ++i_next;
+    if (at_next >= steps) {
+      at_next = wave;
+      ++i_next;
+    }
   };
   static_assert(!kFp8 || 16 * RB * KG <= 64, "a lane per token and step");
 
   // the item that is computed
-  int i = 0, at = from, place = 0;
+  int i = 0, at = wave, place = 0;
   const float *sb = nullptr;
   float score[RB];
   bool chose[RB];
@@ -685,7 +681,7 @@ few_layer_down_kernel(FewLayerArgs p) {
         ++loaded;
       }
     for (int item = 0; item < total; ++item) {
-      if (at == from) {
+      if (at == wave) {
         const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
         if constexpr (kFp8) sb = p.s2 + (static_cast<size_t>(e) * NB + n0 / kScaleBlock) * KB;
 #pragma unroll
@@ -737,8 +733,10 @@ few_layer_down_kernel(FewLayerArgs p) {
         for (int j = 0; j < 4; ++j) acc[b][j] = chose[b] ? fmaf(part[j], s[b], acc[b][j]) : acc[b][j];
       }
       at += kWaves;
-      if (at >= steps) at = wave;
-      if (at == from) ++i;
+      if (at >= steps) {
+        at = wave;
+        ++i;
+      }
     }
   }
 #pragma unroll
