@@ -71,6 +71,8 @@ SIGNATURES = {
     "ccf_rms_norm_backward": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
     "ccf_quantize_rows": (_i, [_p, _i, _i, _i, _p, _p, _p]),
     "ccf_quantize_weight": (_i, [_p, _i, _i, _i, _i, _p, _p, _p]),
+    "ccf_linear_fp8_rows": (_i, [_p, _i, _i, _i, _p, _p, _i, _p, _i, _p, _p, _sz, _p]),
+    "ccf_linear_fp8_workspace_bytes": (_sz, [_i, _i]),
     "ccf_linear_fp8": (_i, [_p, _p, _i, _i, _p, _p, _i, _p, _i, _p, _p]),
     "ccf_ffn1_fp8": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p]),
     "ccf_moe_few_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),

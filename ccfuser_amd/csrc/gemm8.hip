@@ -568,15 +568,23 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
 //
 // 16 TT rows x 16 CT CS columns; KS = 8 / CS wavefronts take every KS-th block of K each, straight from memory, and their
 // sums meet in LDS.  Two blocks are on their way while one is multiplied.
+//
+// In: uint8_t for rows in 8 bits, or half_t or bf16_t for rows that are quantised here, each block of 128 by the four lanes
+// that hold it, to the codes of ccf_quantize_rows.  Every workgroup does that again, but hides it behind its weights' loads,
+// where a launch for it costs 3.5 us.
 template <int TT, int CT, int CS>
 struct SplitShape {
   static constexpr int kWaves = 8, KS = kWaves / CS, BM = 16 * TT, BN = 16 * CT * CS, kLd = BN + 4;
   static constexpr size_t kLds = sizeof(float) * KS * BM * kLd;
 };
 
-template <int TT, int CT, int CS, int kOut>
+template <int TT, int CT, int CS, int kOut, class In>
 __global__ void __launch_bounds__(512, 2)
 gemm8_split_kernel(Gemm8Args p, int n_tiles) {
+  constexpr bool kCodes = sizeof(In) == 1;
+  static_assert(kCodes || TT == 1, "a block of 16 rows is quantised at a time");
+  typedef std::conditional_t<kCodes, half_t, In> Raw;
+  typedef Raw raw8 __attribute__((ext_vector_type(8)));
   using S = SplitShape<TT, CT, CS>;
   using Out = std::conditional_t<kOut == kGemm8Bf16, bf16_t, half_t>;
   extern __shared__ __attribute__((aligned(16))) float s_part[];           // [KS][BM][kLd]
@@ -586,13 +594,13 @@ gemm8_split_kernel(Gemm8Args p, int n_tiles) {
   const int r16 = lane & 15, g = lane >> 4, ks = wave % S::KS, cs = wave / S::KS;
   const int KB = scale_blocks(p.K), NB = scale_blocks(p.N);
   const int rows = tile.rows < S::BM ? tile.rows : S::BM, n0 = tile.n * S::BN, c0 = n0 + cs * 16 * CT;
-  const uint8_t *x[TT];
+  const In *x[TT];
   const float *sa[TT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
     const int r = 16 * t + r16, j = tile.row0 + (r < rows ? r : rows - 1);
     const size_t row = static_cast<size_t>(p.a_rows ? p.a_rows[j] : j);
-    x[t] = p.a + row * p.K + 32 * g;
+    x[t] = reinterpret_cast<const In *>(p.a) + row * p.K + 32 * g;
     sa[t] = p.a_scale + row * KB;
   }
   const uint8_t *w[CT];
@@ -612,6 +620,7 @@ gemm8_split_kernel(Gemm8Args p, int n_tiles) {
 
   const int count = KB > ks ? (KB - ks + S::KS - 1) / S::KS : 0;           // blocks ks, ks + KS, ...
   int8v wf[2][CT], xf[2][TT];
+  raw8 raw[2][4];
   float sf[2][TT];
   auto piece = [&](const uint8_t *q, int kb) {
     const uint8_t *at = q + static_cast<size_t>(kb) * kScaleBlock;
@@ -631,20 +640,51 @@ gemm8_split_kernel(Gemm8Args p, int n_tiles) {
     if ((kb + 1) * kScaleBlock <= p.K) {                                   // uniform
 #pragma unroll
       for (int c = 0; c < CT; ++c) wf[buf][c] = whole(w[c], kb);
+      if constexpr (kCodes) {
 #pragma unroll
-      for (int t = 0; t < TT; ++t) xf[buf][t] = whole(x[t], kb);
+        for (int t = 0; t < TT; ++t) xf[buf][t] = whole(x[t], kb);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) raw[buf][q] = *reinterpret_cast<const raw8 *>(x[0] + static_cast<size_t>(kb) * kScaleBlock + 8 * q);
+      }
     } else {
 #pragma unroll
       for (int c = 0; c < CT; ++c) wf[buf][c] = piece(w[c], kb);
+      if constexpr (kCodes) {
 #pragma unroll
-      for (int t = 0; t < TT; ++t) xf[buf][t] = piece(x[t], kb);
+        for (int t = 0; t < TT; ++t) xf[buf][t] = piece(x[t], kb);
+      } else {
+        const int left = p.K - kb * kScaleBlock - 32 * g;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const In *at = x[0] + static_cast<size_t>(kb) * kScaleBlock + 8 * q;
+          raw[buf][q] = *reinterpret_cast<const raw8 *>(left > 8 * q ? at : reinterpret_cast<const In *>(&kZeros16));
+        }
+      }
     }
 #pragma unroll
-    for (int t = 0; t < TT; ++t) sf[buf][t] = sa[t][kb] * b;
+    for (int t = 0; t < TT; ++t) {
+      if constexpr (kCodes) sf[buf][t] = sa[t][kb] * b;
+      else sf[buf][t] = b;
+    }
+  };
+  auto quantise = [&](auto B_) {                                           // raw[buf] to codes, their scale into sf
+    constexpr int buf = decltype(B_)::value;
+    float top = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) top = fmaxf(top, fabsf(static_cast<float>(raw[buf][q / 8][q % 8])));
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    float inverse;
+    sf[buf][0] = block_scale(top, &inverse) * sf[buf][0];
+    auto v = [&](int q) { return static_cast<float>(raw[buf][q / 8][q % 8]) * inverse; };
+#pragma unroll
+    for (int q = 0; q < 8; ++q) xf[buf][0][q] = pack_fp8(v(4 * q), v(4 * q + 1), v(4 * q + 2), v(4 * q + 3));
   };
   auto multiply = [&](int i, auto B_) {
     constexpr int buf = decltype(B_)::value;
     if (i >= count) return;                                                // uniform
+    if constexpr (!kCodes) quantise(B_);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       float4v part[TT];
@@ -765,10 +805,10 @@ int launch_tiles(const Gemm8Args &p, int part, hipStream_t st, const char *what)
   return check_launch(what);
 }
 
-template <int TT, int CT, int CS, int kOut>
+template <int TT, int CT, int CS, int kOut, class In = uint8_t>
 int launch_split(const Gemm8Args &p, hipStream_t st, const char *what) {
   using S = SplitShape<TT, CT, CS>;
-  auto kernel = gemm8_split_kernel<TT, CT, CS, kOut>;
+  auto kernel = gemm8_split_kernel<TT, CT, CS, kOut, In>;
   const int n_tiles = (p.N + S::BN - 1) / S::BN;
   const long long grid = grid_of(p, S::BM, n_tiles);
   CCF_REQUIRE(grid < (1ll << 28), CCF_ERR_SHAPE, "%s: too many tiles", what);
@@ -847,8 +887,52 @@ int check_product(const Gemm8Args &p, const char *what) {
   return CCF_OK;
 }
 
+// Whether a dense product of rows in 16 bits takes the kernel that quantises them itself: at most 16 rows, cut over K.
+bool quantises(const Gemm8Args &p) {
+  return p.max_rows <= 16 && (g_fp8_form ? g_fp8_form == kSplit : form_of(p) == kSplit);
+}
+
+size_t codes_bytes(int rows, int k) { return (static_cast<size_t>(rows) * k + 255) / 256 * 256; }
+
 }  // namespace
 }  // namespace ccf
+
+extern "C" size_t ccf_linear_fp8_workspace_bytes(int rows, int k) {
+  if (rows <= 0 || k <= 0) return 256;
+  return ccf::codes_bytes(rows, k) + sizeof(float) * rows * ccf::scale_blocks(k);
+}
+
+extern "C" int ccf_linear_fp8_rows(const void *x, int x_dtype, int rows, int k, const void *w_codes, const float *w_scales, int n,
+                                   const void *bias, int dtype, void *y, void *workspace, size_t workspace_bytes, ccf_stream_t stream) {
+  using namespace ccf;
+  CCF_REQUIRE(dtype == CCF_F16 || dtype == CCF_BF16, CCF_ERR_UNSUPPORTED, "linear_fp8: output of type %d", dtype);
+  CCF_REQUIRE(x_dtype == CCF_F16 || x_dtype == CCF_BF16 || x_dtype == CCF_F32, CCF_ERR_UNSUPPORTED, "linear_fp8: rows of type %d", x_dtype);
+  CCF_REQUIRE(rows == 0 || workspace, CCF_ERR_WORKSPACE, "linear_fp8: no workspace");
+  CCF_REQUIRE(aligned16(workspace), CCF_ERR_ARG, "linear_fp8: workspace must be 16-byte aligned");
+  uint8_t *codes = static_cast<uint8_t *>(workspace);
+  Gemm8Args p{codes, nullptr, nullptr, static_cast<const uint8_t *>(w_codes), w_scales, bias, nullptr, rows, 1, n, k, nullptr, y,
+              nullptr, nullptr};
+  float *scales = rows > 0 && k > 0 ? reinterpret_cast<float *>(codes + codes_bytes(rows, k)) : nullptr;
+  p.a_scale = scales;
+  if (int rc = check_product(p, "linear_fp8")) return rc;
+  if (rows == 0) return CCF_OK;
+  CCF_REQUIRE(x, CCF_ERR_ARG, "linear_fp8: null pointer");
+  CCF_REQUIRE(reinterpret_cast<uintptr_t>(x) % (x_dtype == CCF_F32 ? 4 : 2) == 0, CCF_ERR_ARG, "linear_fp8: x is not aligned to its type");
+  CCF_REQUIRE(workspace_bytes >= ccf_linear_fp8_workspace_bytes(rows, k), CCF_ERR_WORKSPACE, "linear_fp8: workspace too small");
+  const hipStream_t st = as_stream(stream);
+  if (x_dtype != CCF_F32 && aligned16(x) && quantises(p)) {
+    p.a = static_cast<const uint8_t *>(x);
+    auto run = [&](auto in, auto out) {
+      return launch_split<1, 4, 1, decltype(out)::value, decltype(in)>(p, st, "linear_fp8");
+    };
+    constexpr std::integral_constant<int, kGemm8Half> half{};
+    constexpr std::integral_constant<int, kGemm8Bf16> bf{};
+    if (x_dtype == CCF_F16) return dtype == CCF_F16 ? run(half_t{}, half) : run(half_t{}, bf);
+    return dtype == CCF_F16 ? run(bf16_t{}, half) : run(bf16_t{}, bf);
+  }
+  if (int rc = launch_quantize_rows(x, rows, k, x_dtype, codes, scales, st)) return rc;
+  return gemm8(p, dtype == CCF_F16 ? kGemm8Half : kGemm8Bf16, st, "linear_fp8");
+}
 
 extern "C" int ccf_linear_fp8(const void *x_codes, const float *x_scales, int rows, int k, const void *w_codes,
                               const float *w_scales, int n, const void *bias, int dtype, void *y, ccf_stream_t stream) {

@@ -774,9 +774,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual:
         raise ValueError("rms_norm: neither y nor its 8-bit form is wanted")
     _same_device(x, weight, residual)
     rows, dev = x.numel() // d, x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_y else None
-    total = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
-    codes = torch.empty(x.shape, dtype=FP8, device=dev) if want_fp8 else None
+    y = torch.empty_like(x) if want_y else None
+    total = torch.empty_like(x) if residual is not None else None
+    codes = torch.empty_like(x, dtype=FP8) if want_fp8 else None
     scale = torch.empty(*x.shape[:-1], _scale_blocks(d), dtype=torch.float32, device=dev) if want_fp8 else None
     rstd = torch.empty(rows, dtype=torch.float32, device=dev) if want_rstd else None
     with _on(x):
@@ -825,7 +825,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError("quantize_rows: x has no columns")
     k = x.shape[-1]
-    codes = torch.empty(x.shape, dtype=FP8, device=x.device)
+    codes = torch.empty_like(x, dtype=FP8)
     scale = torch.empty(*x.shape[:-1], _scale_blocks(k), dtype=torch.float32, device=x.device)
     with _on(x):
         _lib.call("ccf_quantize_rows", _ptr(x), x.numel() // k, k, code, _ptr(codes), _ptr(scale), _stream(x))
@@ -878,12 +878,18 @@ def linear_fp8(x, w_codes: torch.Tensor, w_scale: torch.Tensor, bias: Optional[t
     the call; ``dtype`` is x's unless given) or a pair as ``quantize_rows`` returns it (float16 unless given); the weight is
     [n, k] as ``quantize_weight`` returns it, or any codes with any scale per 128 x 128 block; ``bias`` [n] has y's type.
     k is a multiple of 16, n of 8.  Not differentiable: weights in 8 bits are for serving."""
-    if isinstance(x, torch.Tensor) and dtype is None:
+    raw = isinstance(x, torch.Tensor)
+    if raw and dtype is None:
         dtype = x.dtype
     dtype = torch.float16 if dtype is None else dtype
     if dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"linear_fp8 returns float16 or bfloat16, not {dtype}")
-    codes, scale = _rows_fp8(x, "x")
+    if raw:
+        _check(x, "x", ndim=2)
+        code = _type_code(x, "x")
+        codes = x
+    else:
+        codes, scale = _rows_fp8(x, "x")
     _check_fp8(w_codes, w_scale, "weight", True, 2)
     rows, k = codes.shape
     n = w_codes.shape[0]
@@ -894,10 +900,15 @@ def linear_fp8(x, w_codes: torch.Tensor, w_scale: torch.Tensor, bias: Optional[t
         if bias.shape[0] != n:
             raise ValueError("linear_fp8: bias and weight do not match")
     _same_device(codes, w_codes, bias)
-    y = torch.empty(rows, n, dtype=dtype, device=codes.device)
+    y = torch.empty((rows, n), dtype=dtype, device=codes.device)
     with _on(codes):
-        _lib.call("ccf_linear_fp8", _ptr(codes), _ptr(scale), rows, k, _ptr(w_codes), _ptr(w_scale), n, _ptr(bias),
-                  _TYPE_CODES[dtype], _ptr(y), _stream(codes))
+        if raw:
+            ws = _workspace(_lib.lib().ccf_linear_fp8_workspace_bytes(rows, k), x)
+            _lib.call("ccf_linear_fp8_rows", _ptr(x), code, rows, k, _ptr(w_codes), _ptr(w_scale), n, _ptr(bias), _TYPE_CODES[dtype],
+                      _ptr(y), _ptr(ws), ws.numel(), _stream(x))
+        else:
+            _lib.call("ccf_linear_fp8", _ptr(codes), _ptr(scale), rows, k, _ptr(w_codes), _ptr(w_scale), n, _ptr(bias),
+                      _TYPE_CODES[dtype], _ptr(y), _stream(codes))
     return y
 
 

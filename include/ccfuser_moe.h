@@ -653,6 +653,16 @@ int ccf_linear_fp8(const void *x_codes, const float *x_scales, int rows, int k, 
                    int n, const void *bias, int dtype, void *y, ccf_stream_t stream);
 
 /*
+ * The same from rows [rows, k] in x_dtype (no counterpart in the reference), quantised on the way as ccf_quantize_rows does
+ * it, bit for bit: in the product's own kernel for a few rows, else by a launch in front of it.  x is aligned to its type.
+ */
+int ccf_linear_fp8_rows(const void *x, int x_dtype, int rows, int k, const void *w_codes, const float *w_scales, int n,
+                        const void *bias, int dtype, void *y, void *workspace, size_t workspace_bytes, ccf_stream_t stream);
+
+/* Its workspace (no counterpart in the reference); 16-byte aligned. */
+size_t ccf_linear_fp8_workspace_bytes(int rows, int k);
+
+/*
  * ccf_ffn1_forward in 8 bits: h = gelu(x[src_row[j], :] * w1[e]^T + b1[e]) for offsets[e] <= j < offsets[e+1], left as codes
  * [max_rows, d_ffn] and scales [max_rows, ceil(d_ffn / 128)] of the fp32 value, in expert order.  src_row NULL means row j;
  * w1 codes [E, d_ffn, d_model] with scales per 128 x 128 block, b1 fp16 [E, d_ffn] or NULL.  Rows from offsets[E] on are left

@@ -152,3 +152,30 @@ def test_module_refusals():
     with pytest.raises(ValueError, match="fused"):
         staged.quantize_experts()
     staged.close()
+
+
+@pytest.mark.parametrize("form", [0, 1, 4])
+@pytest.mark.parametrize("rows,k,n", [(1, 2048, 512), (16, 4096, 136), (5, 2080, 264), (16, 48, 8), (17, 2048, 64), (1, 144, 1000)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+def test_product_of_rows_in_16_bits(form, rows, k, n, dt):
+    """The codes that a product makes of its rows are those of ``quantize_rows``, so the results are the same bits; rows of
+    zeros, subnormals, infinities and NaN, and a view that is not 16-byte aligned, among them."""
+    from ccfuser_amd import ops
+    g = torch.Generator().manual_seed(rows + k)
+    x = torch.randn(rows * k + 1, generator=g)
+    x[: k // 2] *= 2.0 ** -20
+    w, s = ops.quantize_weight(torch.randn(n, k, generator=g).cuda())
+    out = torch.bfloat16 if dt == torch.float32 else None
+    ops.set_option("fp8_form", form)
+    try:
+        for at in (0, 1):
+            v = x.to(dt).cuda()[at:at + rows * k].view(rows, k)
+            for special in (None, 0.0, float("inf"), float("nan")):
+                if special is not None:
+                    v = v.clone() if at == 0 else v
+                    v[rows // 2, k // 2] = special
+                want = ops.linear_fp8(ops.quantize_rows(v), w, s, dtype=out or dt)
+                got = ops.linear_fp8(v, w, s, dtype=out)
+                assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    finally:
+        ops.set_option("fp8_form", 0)

@@ -123,3 +123,13 @@ def test_layers_refuse_what_is_their_own(lib):
     assert _layer(lib, s1=None) == 1 and _layer(lib, s2=None) == 1 and _layer(lib, xc=FAKE) == 1
     for f in (lib.ccf_moe_few_workspace_bytes, lib.ccf_moe_fp8_workspace_bytes):
         assert f(4, 64, 64, 4, 2) > 0
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(rows=-1), 1), (dict(k=24), 2), (dict(n=12), 2), (dict(x=None), 1), (dict(x=FAKE + 1), 1), (dict(ws=None), 3), (dict(nbytes=64), 3),
+    (dict(ws=FAKE + 4), 1), (dict(xt=9), 5), (dict(dtype=1), 5), (dict(w=None), 1), (dict(s=None), 1), (dict(y=None), 1)])
+def test_linear_of_16_bit_rows_refuses(lib, bad, code):
+    a = dict(x=FAKE, xt=0, rows=2, k=64, w=FAKE, s=FAKE, n=64, dtype=0, y=FAKE, ws=FAKE, nbytes=1 << 20)
+    a.update(bad)
+    assert lib.ccf_linear_fp8_rows(a["x"], a["xt"], a["rows"], a["k"], a["w"], a["s"], a["n"], None, a["dtype"], a["y"], a["ws"],
+                                   a["nbytes"], None) == code
