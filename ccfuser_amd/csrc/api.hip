@@ -436,7 +436,7 @@ extern "C" int ccf_moe_forward_few(const void *x, const void *wg, const void *bg
   if (tokens == 0) return CCF_OK;
   CCF_REQUIRE(x && wg && w1 && b1 && w2 && b2 && out, CCF_ERR_ARG, "moe_forward_few: null pointer");
   CCF_REQUIRE(few_layer_fits(tokens, d_model, d_ffn, num_expert, top_k), CCF_ERR_SHAPE,
-              "moe_forward_few: %d tokens of %d / %d, top-%d of %d experts: at most 32 tokens, widths a multiple of 64, "
+              "moe_forward_few: %d tokens of %d / %d, top-%d of %d experts: at most 16 tokens, widths a multiple of 64, "
               "top_k <= 8 and num_expert <= 1024 are needed", tokens, d_model, d_ffn, top_k, num_expert);
   CCF_REQUIRE(aligned16(x) && aligned16(wg) && aligned16(w1) && aligned16(w2) && aligned16(out), CCF_ERR_ARG,
               "moe_forward_few: rows must be 16-byte aligned");
@@ -455,7 +455,7 @@ extern "C" size_t ccf_moe_fp8_workspace_bytes(int tokens, int d_model, int d_ffn
   if (tokens < 0 || d_model <= 0 || d_ffn <= 0 || num_expert <= 0 || top_k <= 0) return 0;
   if (static_cast<long long>(tokens) * top_k >= (1ll << 31)) return 0;
   const size_t all = ccf::carve_moe8(nullptr, tokens, d_model, d_ffn, num_expert, top_k).total;
-  const size_t few = tokens <= 32 ? ccf::carve_few(nullptr, tokens, d_ffn, top_k, true).total : 0;
+  const size_t few = tokens <= 16 ? ccf::carve_few(nullptr, tokens, d_ffn, top_k, true).total : 0;
   return all > few ? all : few;
 }
 

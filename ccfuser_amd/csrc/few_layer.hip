@@ -8,7 +8,7 @@
 //
 //   * every workgroup of the first kernel gates for itself: the logits of a few tokens are as long as the launch of a
 //     kernel that would compute them (their sums and the selection are the gate's own, bit for bit);
-//   * no routing: a product's columns are the tokens themselves, 16 or 32 of them, whichever of them chose the expert, so
+//   * no routing: a product's columns are the tokens themselves, 16 of them, whichever of them chose the expert, so
 //     no rows are listed, moved or padded; what a token gets from an expert that it did not choose is dropped;
 //   * the second kernel runs all chosen experts of its 16 columns into one sum, so nothing is left to combine.
 //
@@ -28,7 +28,10 @@
 namespace ccf {
 namespace {
 
-constexpr int kFewTokens = 32;                     // most
+// Most tokens.  With 32 the layer of any size was as fast or faster (17 tokens, us, widths 1024 / 4096, 16 experts: 16 bits 117
+// and 70, 8 bits 72 and 51; 4096 / 14336, 8 experts: 367 and 314, 212 and 213): by then most experts are chosen, and a product
+// that works on all tokens whichever chose the expert moves more of them than of weights.
+constexpr int kFewTokens = 16;
 constexpr int kFewSlots = kFewTokens * kMaxTopK;
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 
@@ -56,7 +59,7 @@ struct Slots {
   unsigned *mask;                                  // [32] of E <= 1024 experts
   int *act, *e;                                    // [n] the chosen experts; the tokens' choice
   float *score;                                    // [n]
-  uint8_t *slot;                                   // [n][32] slot of token t that expert act[i] is, 255: none
+  uint8_t *slot;                                   // [n][16] slot of token t that expert act[i] is, 255: none
 
   __host__ __device__ static int bytes(int n) { return 128 + n * (4 + 4 + 4 + kFewTokens); }
   __device__ __forceinline__ Slots(char *at, int n)
@@ -331,25 +334,25 @@ __device__ __forceinline__ void rows_here(const FewLayerArgs &p, char *s_rows, c
   }
 }
 
-// RB blocks of 16 tokens, of which 8 NX are there.  A workgroup's columns: 16 of fp16 weights, whose K its eight wavefronts
+// At most 8 NX tokens.  A workgroup's columns: 16 of fp16 weights, whose K its eight wavefronts
 // cut among them, 128 in 8 bits, 16 to a wavefront: the columns of a scale of h.  It takes one such unit after the other, the
 // next one's operands on their way.
-template <bool kFp8, int RB, int NX>
+template <bool kFp8, int NX>
 struct UpShape {
   static constexpr int CS = kFp8 ? 8 : 1, KS = kWaves / CS, BN = 16 * CS, kLd = BN + 4;
-  static constexpr int kLoads = 2 + (kFp8 ? 0 : NX * RB), kItem = 1024 * kLoads, kDepth = kFp8 ? 4 : 2;
-  static constexpr int kRing = kWaves * kDepth * kItem, kPart = 4 * KS * 16 * RB * kLd;
+  static constexpr int kLoads = 2 + (kFp8 ? 0 : NX), kItem = 1024 * kLoads, kDepth = kFp8 ? 4 : 2;
+  static constexpr int kRing = kWaves * kDepth * kItem, kPart = 4 * KS * 16 * kLd;
 };
 
-template <bool kFp8, int RB, int NX>
+template <bool kFp8, int NX>
 __global__ void __launch_bounds__(kThreads, 4)
 few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
-  using S = UpShape<kFp8, RB, NX>;
+  using S = UpShape<kFp8, NX>;
   constexpr int KS = S::KS, BN = S::BN, kLd = S::kLd;
   // the rings (first the gate's), part sums, slots, in 8 bits the tokens' codes and scales
   extern __shared__ __attribute__((aligned(1024))) char s_all[];
   const int T = p.tokens, n = T * p.k;
-  float *s_part = reinterpret_cast<float *>(s_all + ring_bytes);           // [KS][16 RB][kLd]
+  float *s_part = reinterpret_cast<float *>(s_all + ring_bytes);           // [KS][16][kLd]
   Slots slots(s_all + ring_bytes + S::kPart, n);
   const RowsLds rows_at = rows_lds(kFp8 ? T : 0, p.d);
   char *s_rows = s_all + ring_bytes + S::kPart + (Slots::bytes(n) + 15) / 16 * 16;
@@ -383,9 +386,9 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
   // this lane's loads: chunk (lane % 8) ^ (row % 8) of row 8 j + lane / 8 of a tile
   const int chunk = (lane & 7) ^ (lane >> 3);
   const uint32_t w_lane = (lane >> 3) * row_bytes + chunk * 16;
-  uint32_t x_lane[RB * NX];
+  uint32_t x_lane[NX];
 #pragma unroll
-  for (int j = 0; j < RB * NX; ++j) {
+  for (int j = 0; j < NX; ++j) {
     const int t = 8 * j + (lane >> 3);             // (two blocks of tokens have all 16 each)
     x_lane[j] = (t < T ? t : T - 1) * row_bytes + chunk * 16;
   }
@@ -417,7 +420,7 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
     if constexpr (!kFp8) {
       const uint8_t *x = reinterpret_cast<const uint8_t *>(p.x) + st * 128;
 #pragma unroll
-      for (int j = 0; j < RB * NX; ++j) load16_to_lds<false>(x, x_lane[j], at + 2048 + 1024 * j);
+      for (int j = 0; j < NX; ++j) load16_to_lds<false>(x, x_lane[j], at + 2048 + 1024 * j);
     }
     ++ahead;
     slot_next = slot_next + 1 < S::kDepth ? slot_next + 1 : 0;
@@ -429,12 +432,12 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
   };
   // the unit that is computed, its item; eight consecutive columns of a token to a thread in its epilogue
   constexpr int kPer = BN / 8;
-  static_assert(16 * RB * kPer <= kThreads, "a thread has at most one piece of the epilogue");
+  static_assert(16 * kPer <= kThreads, "a thread has at most one piece of the epilogue");
   const int t_mine = threadIdx.x / kPer, c_mine = threadIdx.x % kPer * 8;
   int u = blockIdx.x, q = 0, i = 0, n0 = 0, slot = 255, place = 0;
   const float *sb = nullptr;
   half8 bias;
-  float4v acc[RB];
+  float4v acc;
   auto begin = [&]() __attribute__((always_inline)) {
     i = u / blocks;
     const int block = u - i * blocks, e = __builtin_amdgcn_readfirstlane(slots.act[i]);
@@ -443,24 +446,21 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
     slot = t_mine < T && n0 + c_mine < p.f ? slots.of(i, t_mine) : 255;
     bias = half8{0, 0, 0, 0, 0, 0, 0, 0};
     if (slot != 255 && p.b1) bias = *reinterpret_cast<const half8 *>(p.b1 + static_cast<size_t>(e) * p.f + n0 + c_mine);
-#pragma unroll
-    for (int b = 0; b < RB; ++b) acc[b] = float4v{0, 0, 0, 0};
+    acc = float4v{0, 0, 0, 0};
   };
   // the unit's end: the wavefronts' sums meet, GELU, h
   auto finish = [&]() __attribute__((always_inline)) {
     __syncthreads();                               // the last unit's part sums are read
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-      *reinterpret_cast<float4v *>(s_part + (ks * 16 * RB + 16 * b + r16) * kLd + cs * 16 + 4 * g) = acc[b];
+    *reinterpret_cast<float4v *>(s_part + (ks * 16 + r16) * kLd + cs * 16 + 4 * g) = acc;
     __syncthreads();
-    if (t_mine >= 16 * RB) return;
+    if (t_mine >= 16) return;
     const bool mine = slot != 255;
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(bias[j]);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const float *part = s_part + (s * 16 * RB + t_mine) * kLd + c_mine;
+      const float *part = s_part + (s * 16 + t_mine) * kLd + c_mine;
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += part[j];
     }
@@ -503,32 +503,26 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
     place = place + 1 < S::kDepth ? place + 1 : 0;
     const int st = step_of(q);
     const int8v wf = fragment(at, r16, g);
-    int8v xf[RB];
-    float sx[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      if constexpr (kFp8) {
-        const int t = 16 * b + r16 < T ? 16 * b + r16 : T - 1;
-        const char *row = s_rows + t * rows_at.ld + st * 128 + 16 * g;
-        xf[b] = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 64));
-        sx[b] = *reinterpret_cast<const float *>(s_rows + rows_at.scales + 4 * (t * KB + st)) * scalar_load(sb + st);
-      } else {
-        xf[b] = fragment(at + 2048 + 1024 * NX * b, r16 & (8 * NX - 1), g);
-      }
+    int8v xf;
+    float sx;
+    if constexpr (kFp8) {
+      const int t = r16 < T ? r16 : T - 1;
+      const char *row = s_rows + t * rows_at.ld + st * 128 + 16 * g;
+      xf = join(*reinterpret_cast<const int4v *>(row), *reinterpret_cast<const int4v *>(row + 64));
+      sx = *reinterpret_cast<const float *>(s_rows + rows_at.scales + 4 * (t * KB + st)) * scalar_load(sb + st);
+    } else {
+      xf = fragment(at + 2048, r16 & (8 * NX - 1), g);
     }
     reads_done();
     --ahead;
     if (u_next < units) load_item();
     if (count > 0) {                               // uniform
+      const float4v part = product<kFp8>(wf, xf, acc);
+      if constexpr (kFp8) {
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        const float4v part = product<kFp8>(wf, xf[b], acc[b]);
-        if constexpr (kFp8) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[b][j] = fmaf(part[j], sx[b], acc[b][j]);
-        } else {
-          acc[b] = part;
-        }
+        for (int j = 0; j < 4; ++j) acc[j] = fmaf(part[j], sx, acc[j]);
+      } else {
+        acc = part;
       }
     }
     if (++q < turns) continue;
@@ -544,22 +538,22 @@ few_layer_up_kernel(FewLayerArgs p, bool gated, int ring_bytes) {
 // product are CW columns on KG = 16 / CW steps of K at a time, each product with the tokens of one of them: a narrow tile
 // loads as many bytes as a wide one, and there are enough of them for two workgroups on every CU.  A token's results of an
 // expert are scaled by its score (and the blocks' scales) as they are added.
-template <bool kFp8, int RB, int NX, int CW>
+template <bool kFp8, int NX, int CW>
 struct DownShape {
   static constexpr int KG = 16 / CW, kLd = 16 + 4;
-  static constexpr int kLoads = 2 + KG * NX * RB + (kFp8 ? 1 : 0), kItem = 1024 * (2 + KG * NX * RB) + (kFp8 ? 256 : 0);
+  static constexpr int kLoads = 2 + KG * NX + (kFp8 ? 1 : 0), kItem = 1024 * (2 + KG * NX) + (kFp8 ? 256 : 0);
   static constexpr int kDepth = kItem <= 3 * 1024 ? 3 : 2;
-  static constexpr int kRing = kWaves * kDepth * kItem, kPart = 4 * kWaves * 16 * RB * kLd;
+  static constexpr int kRing = kWaves * kDepth * kItem, kPart = 4 * kWaves * 16 * kLd;
 };
 
-template <bool kFp8, int RB, int NX, int CW>
+template <bool kFp8, int NX, int CW>
 __global__ void __launch_bounds__(kThreads, 4)
 few_layer_down_kernel(FewLayerArgs p) {
-  using S = DownShape<kFp8, RB, NX, CW>;
+  using S = DownShape<kFp8, NX, CW>;
   constexpr int KG = S::KG, kLd = S::kLd;
   extern __shared__ __attribute__((aligned(1024))) char s_all[];           // the rings, part sums, slots
   const int T = p.tokens, n = T * p.k;
-  float *s_part = reinterpret_cast<float *>(s_all + S::kRing);             // [wavefronts][16 RB][kLd]
+  float *s_part = reinterpret_cast<float *>(s_all + S::kRing);             // [wavefronts][16][kLd]
   Slots slots(s_all + S::kRing + S::kPart, n);
   for (int q = threadIdx.x; q < n; q += kThreads) {
     const int64_t e = p.idx[q];
@@ -582,7 +576,7 @@ few_layer_down_kernel(FewLayerArgs p) {
 
   // the biases' part of this thread's output
   const int t_mine = threadIdx.x / CW, c_mine = threadIdx.x % CW;
-  static_assert(16 * RB * CW <= kThreads, "a thread has at most one output");
+  static_assert(16 * CW <= kThreads, "a thread has at most one output");
   float sum = 0.0f;
   if (p.b2 && t_mine < T) {
 #pragma unroll 2
@@ -606,20 +600,19 @@ few_layer_down_kernel(FewLayerArgs p) {
   // the item that is loaded next: step `at` of chosen expert `i`, a token that did not choose it taking a row of one that did
   int i_next = 0, at_next = wave, slot_next = 0, ahead = 0;
   const uint8_t *w = nullptr;
-  uint32_t h_lane[RB * NX], s_lane = 0;
+  uint32_t h_lane[NX], s_lane = 0;
   auto aim = [&]() __attribute__((always_inline)) {
     const int e = __builtin_amdgcn_readfirstlane(slots.act[i_next]);
     w = static_cast<const uint8_t *>(p.w2) + (static_cast<size_t>(e) * p.d + n0) * row_bytes;
-    const int t32 = lane & 31, slot32 = t32 < T ? slots.of(i_next, t32) : 255;
-    const int row32 = t32 * p.k + slot32;
-    const int some = __builtin_amdgcn_readlane(row32, __ffsll(__ballot(slot32 != 255)) - 1);
+    const int t16 = lane & 15, slot16 = t16 < T ? slots.of(i_next, t16) : 255;
+    const int some = __builtin_amdgcn_readlane(t16 * p.k + slot16, __ffsll(__ballot(slot16 != 255)) - 1);
     auto row_of = [&](int t) {
       const int slot = t < T ? slots.of(i_next, t) : 255;
       return static_cast<uint32_t>(slot != 255 ? t * p.k + slot : some);
     };
 #pragma unroll
-    for (int j = 0; j < RB * NX; ++j) h_lane[j] = row_of(8 * j + (lane >> 3)) * row_bytes + chunk * 16;
-    if constexpr (kFp8) s_lane = row_of(lane % (16 * RB)) * KB;
+    for (int j = 0; j < NX; ++j) h_lane[j] = row_of(8 * j + (lane >> 3)) * row_bytes + chunk * 16;
+    if constexpr (kFp8) s_lane = row_of(lane % (16)) * KB;
   };
   auto load_item = [&]() __attribute__((always_inline)) {
     if (at_next == wave) aim();
@@ -642,17 +635,17 @@ few_layer_down_kernel(FewLayerArgs p) {
 #pragma unroll
     for (int k = 0; k < KG; ++k)
 #pragma unroll
-      for (int j = 0; j < RB * NX; ++j) {
-        const uint32_t to = at + 2048 + 1024 * (k * RB * NX + j);
+      for (int j = 0; j < NX; ++j) {
+        const uint32_t to = at + 2048 + 1024 * (k * NX + j);
         if (left < 128 * KG)
           load16_to_lds(128 * k + chunk * 16 < left ? h + (128 * k + h_lane[j]) : reinterpret_cast<const uint8_t *>(&kZeros16), to);
         else
           load16_to_lds<false>(h + 128 * k, h_lane[j], to);
       }
     if constexpr (kFp8) {
-      // the scales of the tokens at the item's steps, token t at step k in lane 16 RB k + t
-      const int k = lane / (16 * RB) < KG ? lane / (16 * RB) : KG - 1, kb = at_next * KG + k < KB ? at_next * KG + k : KB - 1;
-      load4_to_lds(p.h_scales, 4 * (s_lane + kb), at + 1024 * (2 + KG * NX * RB));
+      // the scales of the tokens at the item's steps, token t at step k in lane 16 k + t
+      const int k = lane / (16) < KG ? lane / (16) : KG - 1, kb = at_next * KG + k < KB ? at_next * KG + k : KB - 1;
+      load4_to_lds(p.h_scales, 4 * (s_lane + kb), at + 1024 * (2 + KG * NX));
     }
     ++ahead;
     slot_next = slot_next + 1 < S::kDepth ? slot_next + 1 : 0;
@@ -662,16 +655,14 @@ few_layer_down_kernel(FewLayerArgs p) {
       ++i_next;
     }
   };
-  static_assert(!kFp8 || 16 * RB * KG <= 64, "a lane per token and step");
+  static_assert(!kFp8 || 16 * KG <= 64, "a lane per token and step");
 
   // the item that is computed
   int i = 0, at = wave, place = 0;
   const float *sb = nullptr;
-  float score[RB];
-  bool chose[RB];
-  float4v acc[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) acc[b] = float4v{0, 0, 0, 0};
+  float score;
+  bool chose;
+  float4v acc = float4v{0, 0, 0, 0};
   if (total > 0) {
     int loaded = 0;
 #pragma unroll
@@ -684,36 +675,30 @@ few_layer_down_kernel(FewLayerArgs p) {
       if (at == wave) {
         const int e = __builtin_amdgcn_readfirstlane(slots.act[i]);
         if constexpr (kFp8) sb = p.s2 + (static_cast<size_t>(e) * NB + n0 / kScaleBlock) * KB;
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          const int t = 16 * b + r16, slot = t < T ? slots.of(i, t) : 255;
-          chose[b] = slot != 255;
-          score[b] = chose[b] ? slots.score[t * p.k + slot] : 0.0f;
-        }
+        const int t = r16, slot = t < T ? slots.of(i, t) : 255;
+        chose = slot != 255;
+        score = chose ? slots.score[t * p.k + slot] : 0.0f;
       }
       if (ahead == S::kDepth) loads_but<S::kLoads *(S::kDepth - 1)>();
       else loads_but<0>();
       const char *tile = ring + place * S::kItem;
       place = place + 1 < S::kDepth ? place + 1 : 0;
       const int8v wf = fragment(tile, r16, g);
-      int8v hf[RB][KG];
-      float s[RB];
+      int8v hf[KG];
+      float s;
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
+      for (int k = 0; k < KG; ++k)
+        hf[k] = fragment(tile + 2048 + 1024 * NX * k, r16 & (8 * NX - 1), g);
+      s = score;
+      if constexpr (kFp8) {
+        // (weights' scales of all the item's steps, this lane's picked)
+        float scale = scalar_load(sb + at * KG);
 #pragma unroll
-        for (int k = 0; k < KG; ++k)
-          hf[b][k] = fragment(tile + 2048 + 1024 * NX * (k * RB + b), r16 & (8 * NX - 1), g);
-        s[b] = score[b];
-        if constexpr (kFp8) {
-          // (weights' scales of all the item's steps, this lane's picked)
-          float scale = scalar_load(sb + at * KG);
-#pragma unroll
-          for (int k = 1; k < KG; ++k) {
-            const float other = scalar_load(sb + (at * KG + k < KB ? at * KG + k : KB - 1));
-            scale = mine_k == k ? other : scale;
-          }
-          s[b] *= *reinterpret_cast<const float *>(tile + 1024 * (2 + KG * NX * RB) + 4 * (16 * RB * mine_k + 16 * b + r16)) * scale;
+        for (int k = 1; k < KG; ++k) {
+          const float other = scalar_load(sb + (at * KG + k < KB ? at * KG + k : KB - 1));
+          scale = mine_k == k ? other : scale;
         }
+        s *= *reinterpret_cast<const float *>(tile + 1024 * (2 + KG * NX) + 4 * (16 * mine_k + r16)) * scale;
       }
       reads_done();
       --ahead;
@@ -721,17 +706,14 @@ few_layer_down_kernel(FewLayerArgs p) {
         load_item();
         ++loaded;
       }
+      float4v part = product<kFp8>(wf, hf[0]);
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        float4v part = product<kFp8>(wf, hf[b][0]);
-#pragma unroll
-        for (int k = 1; k < KG; ++k) {
-          const float4v other = product<kFp8>(wf, hf[b][k]);
-          part = mine_k == k ? other : part;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[b][j] = chose[b] ? fmaf(part[j], s[b], acc[b][j]) : acc[b][j];
+      for (int k = 1; k < KG; ++k) {
+        const float4v other = product<kFp8>(wf, hf[k]);
+        part = mine_k == k ? other : part;
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = chose ? fmaf(part[j], s, acc[j]) : acc[j];
       at += kWaves;
       if (at >= steps) {
         at = wave;
@@ -739,14 +721,13 @@ few_layer_down_kernel(FewLayerArgs p) {
       }
     }
   }
-#pragma unroll
-  for (int b = 0; b < RB; ++b) *reinterpret_cast<float4v *>(s_part + (wave * 16 * RB + 16 * b + r16) * kLd + 4 * g) = acc[b];
+  *reinterpret_cast<float4v *>(s_part + (wave * 16 + r16) * kLd + 4 * g) = acc;
   __syncthreads();
   if (t_mine < T) {
 #pragma unroll
     for (int x = 0; x < kWaves; ++x)
 #pragma unroll
-      for (int j = 0; j < KG; ++j) sum += s_part[(x * 16 * RB + t_mine) * kLd + j * CW + c_mine];
+      for (int j = 0; j < KG; ++j) sum += s_part[(x * 16 + t_mine) * kLd + j * CW + c_mine];
     p.out[static_cast<size_t>(t_mine) * p.d + n0 + c_mine] = static_cast<half_t>(sum);
   }
 }
@@ -767,13 +748,13 @@ int allow_lds(K kernel, size_t lds) {
   return e == hipSuccess ? static_cast<int>(CCF_OK) : fail(CCF_ERR_HIP, "few_layer: LDS attribute: %s", hipGetErrorString(e));
 }
 
-template <bool kFp8, int RB, int NX>
+template <bool kFp8, int NX>
 int launch_up(const FewLayerArgs &p, bool gated, size_t gate_bytes, hipStream_t st) {
-  using S = UpShape<kFp8, RB, NX>;
+  using S = UpShape<kFp8, NX>;
   const int n = p.tokens * p.k;
   const size_t ring = gate_bytes > S::kRing ? (gate_bytes + 1023) / 1024 * 1024 : S::kRing;
   const size_t lds = ring + S::kPart + (Slots::bytes(n) + 15) / 16 * 16 + (kFp8 ? rows_lds(p.tokens, p.d).bytes : 0);
-  auto kernel = few_layer_up_kernel<kFp8, RB, NX>;
+  auto kernel = few_layer_up_kernel<kFp8, NX>;
   if (int rc = allow_lds(kernel, lds)) return rc;
   const long long units = static_cast<long long>(p.E < n ? p.E : n) * ((p.f + S::BN - 1) / S::BN);
   const int most = lds > 80 * 1024 ? 256 : 512;                // workgroups on the chip at once
@@ -782,42 +763,37 @@ int launch_up(const FewLayerArgs &p, bool gated, size_t gate_bytes, hipStream_t 
   return check_launch("few_layer_up_kernel");
 }
 
-template <bool kFp8, int RB, int NX, int CW>
+template <bool kFp8, int NX, int CW>
 int launch_down_at(const FewLayerArgs &p, hipStream_t st) {
-  using S = DownShape<kFp8, RB, NX, CW>;
+  using S = DownShape<kFp8, NX, CW>;
   const size_t lds = S::kRing + S::kPart + Slots::bytes(p.tokens * p.k);
-  auto kernel = few_layer_down_kernel<kFp8, RB, NX, CW>;
+  auto kernel = few_layer_down_kernel<kFp8, NX, CW>;
   if (int rc = allow_lds(kernel, lds)) return rc;
   hipLaunchKernelGGL(kernel, dim3(p.d / CW), dim3(kThreads), lds, st, p);
   return check_launch("few_layer_down_kernel");
 }
 
-template <bool kFp8, int RB, int NX>
+template <bool kFp8, int NX>
 int launch_down(const FewLayerArgs &p, hipStream_t st) {
-  // the widest tiles of which there are two for every CU; more tokens have items of their own size with wide ones
-  if constexpr (RB == 1 && NX == 1) {
-    if (p.d < 8 * 256) return launch_down_at<kFp8, RB, NX, 4>(p, st);
+  // the widest tiles of which there are two for every CU; with more than 8 tokens an item of narrow ones is mostly tokens
+  if constexpr (NX == 1) {
+    if (p.d < 8 * 256) return launch_down_at<kFp8, NX, 4>(p, st);
   }
-  if constexpr (RB == 1) {
-    if (p.d < 16 * 512) return launch_down_at<kFp8, RB, NX, 8>(p, st);
-  }
-  return launch_down_at<kFp8, RB, NX, 16>(p, st);
+  return p.d < 16 * 512 ? launch_down_at<kFp8, NX, 8>(p, st) : launch_down_at<kFp8, NX, 16>(p, st);
 }
 
 template <bool kFp8>
 int launch_few_layer(const FewLayerArgs &p, bool gated, size_t gate_bytes, hipStream_t st) {
-  auto run = [&](auto RB_, auto NX_) {
-    constexpr int RB = decltype(RB_)::value, NX = decltype(NX_)::value;
-    if (int rc = launch_up<kFp8, RB, NX>(p, gated, gate_bytes, st)) return rc;
-    return launch_down<kFp8, RB, NX>(p, st);
+  auto run = [&](auto NX_) {
+    constexpr int NX = decltype(NX_)::value;
+    if (int rc = launch_up<kFp8, NX>(p, gated, gate_bytes, st)) return rc;
+    return launch_down<kFp8, NX>(p, st);
   };
-  using One = std::integral_constant<int, 1>;
-  using Two = std::integral_constant<int, 2>;
-  return p.tokens <= 8 ? run(One{}, One{}) : (p.tokens <= 16 ? run(One{}, Two{}) : run(Two{}, Two{}));
+  return p.tokens <= 8 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
 }
 
-// What the first kernel may keep in LDS of the gate's operands, and of tokens in 8 bits beside its rings, part sums (17 KB at
-// most) and slots (11 KB).
+// What the first kernel may keep in LDS of the gate's operands, and of tokens in 8 bits beside its rings, part sums (9 KB at
+// most) and slots (4 KB).
 constexpr int kMaxGateLds = 64 * 1024, kMaxRowsLds = 64 * 1024;
 
 }  // namespace

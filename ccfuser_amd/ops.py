@@ -972,6 +972,7 @@ def ffn2_fp8(h, dst_row: Optional[torch.Tensor], offsets: torch.Tensor, max_rows
 
 
 FEW_TOKENS = 32              # most tokens of ``moe_forward_few``
+_FEW_KERNEL_TOKENS = 16      # most of them in the two kernels
 
 
 def _check_layer(x, wg, bg, top_k: int, what: str) -> None:
@@ -990,9 +991,9 @@ def _check_layer(x, wg, bg, top_k: int, what: str) -> None:
 def moe_forward_few(x: torch.Tensor, wg: torch.Tensor, bg: Optional[torch.Tensor], w1: torch.Tensor, b1: torch.Tensor,
                     w2: torch.Tensor, b2: torch.Tensor, top_k: int, return_routing: bool = False,
                     workspace: Optional[torch.Tensor] = None, spare_experts: bool = False):
-    """``moe_forward`` for at most 32 tokens in two kernels: out [T, d] fp16 (and ``idx`` and ``score`` on request).  The
-    choice is the gate's, bit for bit; outputs differ from ``moe_forward``'s in the order of sums and by one rounding.
-    ``spare_experts`` as in ``moe_forward``."""
+    """``moe_forward`` for at most 32 tokens: out [T, d] fp16 (and ``idx`` and ``score`` on request).  Up to 16 tokens take two
+    kernels, whose choice is the gate's, bit for bit, and whose outputs differ from ``moe_forward``'s in the order of sums and
+    by one rounding; more take ``moe_forward``'s own, which are faster there.  ``spare_experts`` as in ``moe_forward``."""
     top_k = int(top_k)
     _check_layer(x, wg, bg, top_k, "moe_forward_few")
     _check_expert(w1, b1, "ffn1")
@@ -1004,6 +1005,9 @@ def moe_forward_few(x: torch.Tensor, wg: torch.Tensor, bg: Optional[torch.Tensor
         raise ValueError("moe_forward_few: weight shapes do not match")
     if T > FEW_TOKENS:
         raise ValueError(f"moe_forward_few takes at most {FEW_TOKENS} tokens, got {T}")
+    if T > _FEW_KERNEL_TOKENS:
+        return moe_forward(x, wg, bg, w1, b1, w2, b2, top_k, return_routing=return_routing, workspace=workspace,
+                           spare_experts=spare_experts)
     _same_device(x, wg, bg, w1, b1, w2, b2, workspace)
     out = torch.empty_like(x)
     idx = torch.empty(T, top_k, dtype=torch.int64, device=x.device) if return_routing else None

@@ -687,7 +687,7 @@ size_t ccf_moe_few_workspace_bytes(int tokens, int d_model, int d_ffn, int num_e
  * ccf_moe_forward for a few tokens in two kernels: gate, choice, FFN1 and GELU; FFN2 and the combine
  * (mix_moe/csrc/mix_moe.h:507-598).  The choice and its scores are the gate's, bit for bit; the outputs come of other sums
  * than ccf_moe_forward's and one rounding less (an expert's output is not rounded to fp16 before the combine).
- * At most 32 tokens, widths a multiple of 64, no capacity limit (an expert gets as many rows as there are tokens at most).
+ * At most 16 tokens, widths a multiple of 64, no capacity limit (an expert gets as many rows as there are tokens at most).
  * With more experts, tokens or a wider model than a workgroup gates for itself, the gate is a launch in front.
  * idx_out int64 [tokens*top_k] (-1: no expert), score_out fp16 [tokens*top_k], NULL to skip.
  */
@@ -699,7 +699,7 @@ int ccf_moe_forward_few(const void *x, const void *wg, const void *bg, const voi
 size_t ccf_moe_fp8_workspace_bytes(int tokens, int d_model, int d_ffn, int num_expert, int top_k);
 
 /*
- * ccf_moe_forward on experts in 8 bits: gate in fp16, ccf_ffn1_fp8, ccf_ffn2_fp8, combine; at most 32 tokens in the two
+ * ccf_moe_forward on experts in 8 bits: gate in fp16, ccf_ffn1_fp8, ccf_ffn2_fp8, combine; at most 16 tokens in the two
  * kernels of ccf_moe_forward_few (mix_moe/csrc/mix_moe.h:507-598 in fp16).
  *   x [tokens, d_model] fp16 is what the gate scores; x_codes and x_scales, the same rows in 8 bits for the experts, may be
  *   NULL (quantised by the call).  Weights as in ccf_ffn1_fp8 and ccf_ffn2_fp8, b1 and b2 fp16 or NULL; capacity as in
