@@ -438,7 +438,7 @@ extern "C" int ccf_moe_forward_few(const void *x, const void *wg, const void *bg
   CCF_REQUIRE(few_layer_fits(tokens, d_model, d_ffn, num_expert, top_k), CCF_ERR_SHAPE,
               "moe_forward_few: %d tokens of %d / %d, top-%d of %d experts: at most 16 tokens, widths a multiple of 64, "
               "top_k <= 8 and num_expert <= 1024 are needed", tokens, d_model, d_ffn, top_k, num_expert);
-  CCF_REQUIRE(aligned16(x) && aligned16(wg) && aligned16(w1) && aligned16(w2) && aligned16(out), CCF_ERR_ARG,
+  CCF_REQUIRE(aligned16(x) && aligned16(wg) && aligned16(w1) && aligned16(w2) && aligned16(b1) && aligned16(b2) && aligned16(out), CCF_ERR_ARG,
               "moe_forward_few: rows must be 16-byte aligned");
   const size_t need = ccf_moe_few_workspace_bytes(tokens, d_model, d_ffn, num_expert, top_k);
   CCF_REQUIRE(workspace && workspace_bytes >= need, CCF_ERR_WORKSPACE, "moe_forward_few: workspace of %zu bytes needed, %zu given",
@@ -476,6 +476,11 @@ extern "C" int ccf_moe_forward_fp8(const void *x, const void *x_codes, const flo
               "moe_forward_fp8: null pointer");
   CCF_REQUIRE(aligned16(x) && aligned16(x_codes) && aligned16(wg) && aligned16(w1_codes) && aligned16(w2_codes) && aligned16(out) &&
                   aligned16(b1) && aligned16(b2), CCF_ERR_ARG, "moe_forward_fp8: rows must be 16-byte aligned");
+  // (what the products count in 32 bits)
+  const long long widest = d_model > d_ffn ? d_model : d_ffn;
+  CCF_REQUIRE(static_cast<long long>(tokens) * top_k < (1 << 30) && static_cast<long long>(tokens) * top_k * (widest / 16) < (1ll << 32) &&
+                  static_cast<long long>(d_model) * d_ffn < (1ll << 32), CCF_ERR_SHAPE,
+              "moe_forward_fp8: %d tokens of %d / %d, top-%d: a matrix too large", tokens, d_model, d_ffn, top_k);
   const size_t need = ccf_moe_fp8_workspace_bytes(tokens, d_model, d_ffn, num_expert, top_k);
   CCF_REQUIRE(workspace && workspace_bytes >= need, CCF_ERR_WORKSPACE, "moe_forward_fp8: workspace of %zu bytes needed, %zu given",
               need, workspace_bytes);

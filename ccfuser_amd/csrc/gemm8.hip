@@ -834,7 +834,10 @@ Form form_of(const Gemm8Args &p) {
   const long long rows = (p.max_rows + owners - 1) / owners, likely = grouped ? rows + rows / 4 : rows;
   auto tiles = [&](int bm, int bn) { return owners * ((likely + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   if (p.K >= 2048 && (grouped ? 2 * rows : rows) <= 32 && owners * ((p.N + 63) / 64) <= kCus) return kSplit;
-  if (owners * (rows / kWholeRows) * ((p.N + 255) / 256) >= kCus) return kTilesAndRest;
+  if (owners * (rows / kWholeRows) * ((p.N + 255) / 256) >= kCus) {
+    const long long rest = rows % kWholeRows;
+    return grouped || (rest > 0 && rest <= kLeftRows) ? kTilesAndRest : kTiles256;          // an empty launch is 4 us
+  }
   if (likely <= 64 || tiles(64, 128) <= 448) return kTiles64;
   if (likely > 128 && tiles(128, 128) >= 640) return kTiles256;
   return kTiles128;

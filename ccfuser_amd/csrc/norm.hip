@@ -13,6 +13,10 @@
 // One pass: a row stays in the registers of its threads (8 consecutive elements each, 16 lanes to a scale's block) between
 // the loads, the sum and the stores.  Rows too long for that are read again.  The backward keeps a thread's columns of the
 // weight gradient in registers over all rows of a workgroup, and a second launch adds the workgroups' sums in order.
+//
+// Measured, bf16 with a residual, 16384 x 4096: forward 98.8 us, 5.4 TB/s (1 GiB copied: 5.1); backward with both gradients
+// 139.7 us, 3.8 TB/s (of its four streams one is written); quantize_rows 31.9 us, 6.3 TB/s.  8 x 14336 x 4096 fp16 weights to
+// 8 bits 279 us, 5.1 TB/s.  One row of 4096: 3.9, 6.5 and 2.8 us, a launch's own time.
 #include "fp8.h"
 
 #include <type_traits>

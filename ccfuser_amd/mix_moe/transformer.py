@@ -256,13 +256,14 @@ class MixMOETransformerMLP(MixMOE):
         up, down = self.experts.htoh4.weight, self.experts.h4toh.weight
         E = self.num_expert
         self._experts8 = (*ops.quantize_weight(up.detach()[:E].contiguous()), *ops.quantize_weight(down.detach()[:E].contiguous()),
-                          (up._version, down._version))
+                          (up, up._version, down, down._version))
         return self
 
     def _forward_fp8(self, inp):
-        w1, s1, w2, s2, versions = self._experts8
+        w1, s1, w2, s2, (w_up, up_version, w_down, down_version) = self._experts8
         lin, up, down = self.gate.gate, self.experts.htoh4, self.experts.h4toh
-        if (up.weight._version, down.weight._version) != versions:
+        if not (up.weight is w_up and up.weight._version == up_version and
+                down.weight is w_down and down.weight._version == down_version):
             raise RuntimeError("expert weights have changed since quantize_experts()")
         x_fp8 = None
         if self.norm is not None:

@@ -77,6 +77,10 @@ def test_module_on_experts_in_8_bits(T, pre_norm):
             mlp(l["x"])
         mlp.experts.htoh4.weight.mul_(0.5)
         assert torch.equal(mlp.quantize_experts()(l["x"]), out)
+        mlp.quantize_experts()
+        mlp.experts.h4toh.weight = torch.nn.Parameter(mlp.experts.h4toh.weight.clone())
+        with pytest.raises(RuntimeError, match="changed"):
+            mlp(l["x"])
         assert torch.equal(mlp.quantize_experts(False)(l["x"]), before)
     mlp.close()
 
@@ -179,3 +183,36 @@ def test_product_of_rows_in_16_bits(form, rows, k, n, dt):
                 assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
     finally:
         ops.set_option("fp8_form", 0)
+
+
+def test_product_of_no_rows():
+    from ccfuser_amd import ops
+    w, s = ops.quantize_weight(torch.randn(64, 128).half().cuda())
+    x = torch.empty(0, 128, dtype=torch.float16, device="cuda")
+    for rows in (x, ops.quantize_rows(x)):
+        assert ops.linear_fp8(rows, w, s).shape == (0, 64)
+    l = _layer(1, 64, 64, 2, 1)
+    q = [t for n in ("w1", "w2") for t in ops.quantize_weight(l[n])]
+    none = l["x"][:0]
+    assert ops.moe_forward_few(none, *list(l.values())[1:], 1).shape == (0, 64)
+    assert ops.moe_forward_fp8(none, l["wg"], l["bg"], q[0], q[1], l["b1"], q[2], q[3], l["b2"], 1).shape == (0, 64)
+
+
+def test_two_products_at_once():
+    """Calls on two streams share nothing: each result is the one that the call gives alone."""
+    from ccfuser_amd import ops
+    g = torch.Generator().manual_seed(3)
+    w, s = ops.quantize_weight(torch.randn(2048, 2048, generator=g).half().cuda())
+    xs = [torch.randn(r, 2048, generator=g).half().cuda() for r in (3, 16, 40, 700)]
+    l = _layer(9, 256, 512, 8, 2, seed=120)
+    args = [l[n] for n in ("x", "wg", "bg", "w1", "b1", "w2", "b2")]
+    alone = [ops.linear_fp8(x, w, s) for x in xs] + [ops.moe_forward_few(*args, 2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for i in range(5):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append(ops.linear_fp8(xs[i], w, s) if i < 4 else ops.moe_forward_few(*args, 2))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, alone))

@@ -103,7 +103,7 @@ def _layer(lib, **bad):
 
 
 def _few(lib, **bad):
-    a = dict(x=FAKE, wg=FAKE, bg=None, w1=FAKE, b1=None, w2=FAKE, b2=None, out=FAKE, ws=FAKE, nbytes=1 << 30, **LAYER)
+    a = dict(x=FAKE, wg=FAKE, bg=None, w1=FAKE, b1=FAKE, w2=FAKE, b2=FAKE, out=FAKE, ws=FAKE, nbytes=1 << 30, **LAYER)
     a.update(bad)
     return lib.ccf_moe_forward_few(a["x"], a["wg"], a["bg"], a["w1"], a["b1"], a["w2"], a["b2"], a["T"], a["d"], a["f"], a["E"], a["k"],
                                    a["out"], None, None, a["ws"], a["nbytes"], None)
@@ -119,7 +119,9 @@ def test_layers_refuse(lib, bad):
 
 
 def test_layers_refuse_what_is_their_own(lib):
-    assert _few(lib, T=33) != 0
+    assert _few(lib, T=17) == 2
+    assert _layer(lib, T=1 << 29, nbytes=1 << 62) == 2 and _layer(lib, T=1 << 24, f=1 << 16, nbytes=1 << 62) == 2
+    assert _layer(lib, d=1 << 17, f=1 << 15, nbytes=1 << 62) == 2
     assert _layer(lib, s1=None) == 1 and _layer(lib, s2=None) == 1 and _layer(lib, xc=FAKE) == 1
     for f in (lib.ccf_moe_few_workspace_bytes, lib.ccf_moe_fp8_workspace_bytes):
         assert f(4, 64, 64, 4, 2) > 0
