@@ -17,15 +17,23 @@ class _RMSNorm(torch.autograd.Function):
         return (n.y, n.total) if residual is not None else n.y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y, grad_total=None):
-        total, weight, rstd = ctx.saved_tensors
-        need_x, need_w, _, need_r = ctx.needs_input_grad
-        if grad_y is None:                               # y was not used
-            return grad_total if need_x else None, None, None, grad_total if need_r else None
-        g_x, g_w = ops.rms_norm_backward(grad_y.contiguous(), total, weight, rstd,
-                                         None if grad_total is None else grad_total.contiguous(), need_x or need_r, need_w)
-        return g_x if need_x else None, g_w, None, g_x if need_r else None
+        # (the decorator costs as much host time as a launch, and says nothing where no graph is made of the backward)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_y, grad_total)
+
+
+def _backward(ctx, grad_y, grad_total):
+    total, weight, rstd = ctx.saved_tensors
+    need_x, need_w, _, need_r = ctx.needs_input_grad
+    if grad_y is None:                                   # y was not used
+        return grad_total if need_x else None, None, None, grad_total if need_r else None
+    # shapes and types are the forward's, which it checked
+    g_x, g_w = ops._rms_norm_backward(grad_y.contiguous(), total, weight, rstd, None if grad_total is None else grad_total.contiguous(),
+                                      need_x or need_r, need_w, ops._type_code(total, "total"))
+    return g_x if need_x else None, g_w, None, g_x if need_r else None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 def rms_norm(x, weight, eps=1e-5, residual=None):

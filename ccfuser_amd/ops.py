@@ -807,6 +807,12 @@ def rms_norm_backward(grad_y: torch.Tensor, total: torch.Tensor, weight: torch.T
     _same_device(total, grad_y, weight, rstd, grad_total)
     if not (want_x or want_weight):
         return None, None
+    return _rms_norm_backward(grad_y, total, weight, rstd, grad_total, want_x, want_weight, code)
+
+
+def _rms_norm_backward(grad_y, total, weight, rstd, grad_total, want_x, want_weight, code):
+    """``rms_norm_backward`` behind its checks."""
+    d = weight.shape[0]
     rows = total.numel() // d
     g_x = torch.empty_like(total) if want_x else None
     g_w = torch.empty_like(weight) if want_weight else None

@@ -216,3 +216,17 @@ def test_two_products_at_once():
                 got.append(ops.linear_fp8(xs[i], w, s) if i < 4 else ops.moe_forward_few(*args, 2))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, alone))
+
+
+def test_norm_is_differentiable_once():
+    """A graph of the backward may be asked for, and what it holds of the norm is refused, not taken for a constant."""
+    from ccfuser_amd.mix_moe import rms_norm
+    x = torch.randn(4, 64).half().cuda().requires_grad_()
+    w = torch.ones(64).half().cuda().requires_grad_()
+    y = rms_norm(x, w)
+    g = torch.randn_like(y).requires_grad_()
+    plain = torch.autograd.grad(y, (x, w), g, retain_graph=True)
+    first = torch.autograd.grad(y, (x, w), g, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, first))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first[0].sum().backward()
