@@ -1863,7 +1863,7 @@ extern "C" int ccf_set_option(const char *name, int value) {
     return CCF_OK;
   }
   if (!strcmp(name, "fp8_form")) {           // products in 8 bits: 0 by the rule, 1 K cut over the wavefronts, 2 tiles in LDS
-    CCF_REQUIRE(value >= 0 && value <= 5, CCF_ERR_ARG, "set_option: fp8_form %d outside 0..5", value);
+    CCF_REQUIRE(value >= 0 && value <= 6, CCF_ERR_ARG, "set_option: fp8_form %d outside 0..6", value);
     g_fp8_form = value;
     return CCF_OK;
   }

@@ -22,7 +22,7 @@ struct Gemm8Args {
 
 enum { kGemm8Half = 0, kGemm8Bf16 = 1, kGemm8Gelu8 = 2 };     // the output: fp16, bf16, or GELU and 8 bits
 
-extern int g_fp8_form;       // ccf_set_option("fp8_form"): 0 .. 5
+extern int g_fp8_form;       // ccf_set_option("fp8_form"): 0 .. 6
 
 int gemm8(const Gemm8Args &p, int out, hipStream_t stream, const char *what);
 

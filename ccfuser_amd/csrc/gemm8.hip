@@ -112,15 +112,18 @@ __device__ __forceinline__ Tile find_tile(const Gemm8Args &p, int pid, int grid,
 // in front of its last columns, whose fragment is in registers by then: behind it this step's place is free for the loads
 // of the step after the next, and the next step's rows are read between the last products, each into the registers that a
 // product has just let go.  So the matrix cores run through the steps, and a load has a whole step to land.
-template <int BM, int BN, int WM, int WN, int NS>
+//
+// KS = 2: two groups of such wavefronts take every other block each, with places of their own, and their sums meet in LDS at
+// the tile's end: half as many steps, for a CU that has one small tile.
+template <int BM, int BN, int WM, int WN, int NS, int KS>
 struct TileShape {
-  static constexpr int kPlaces = NS;
-  static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
+  static constexpr int kWaves = WM * WN, kThreads = KS * kWaves * 64;       // (wavefronts of a group)
   static constexpr int TT = BM / WM / 16, CT = BN / WN / 16;       // 16 x 16 products of a wavefront: rows, columns
   static constexpr int kRowsBytes = (BM + BN) * kScaleBlock;       // a place: codes, then scales of rows, then of columns
   static constexpr int kStage = kRowsBytes + 4 * (BM + 64);
   static constexpr int kLoadsX = BM / 8 / kWaves, kLoadsW = BN / 8 / kWaves;      // loads of 1 KB per wavefront and step
   static constexpr int kLoads = kLoadsX + kLoadsW;
+  static constexpr int kPlace = KS * kStage, kMeet = KS > 1 ? 4 * BM * BN : 0, kMap = NS * kPlace + kMeet;
   static_assert(kWaves >= BM / 64 + 1, "a wavefront more than the rows' scales take loads the columns'");
 };
 
@@ -249,22 +252,22 @@ __device__ __forceinline__ void tile_sources(const Gemm8Args &p, const Tile &til
   }
 }
 
-// On to the step behind `next`'s next_kb, which is loaded; e < 0: there is none.
-template <class S, int BM, int BN>
-__device__ __forceinline__ void advance(const Gemm8Args &p, const TileMap<BM> &map, int end, int slots, int wave, int lane, int chunk,
-                                        int KB, int NB, Tile &next, int &next_kb, int &t_next, int &ahead,
+// On to the step behind `next`'s next_step, which is loaded; e < 0: there is none.
+template <class S, int BM, int BN, int KS>
+__device__ __forceinline__ void advance(const Gemm8Args &p, const TileMap<BM> &map, int end, int slots, int ks, int wave, int lane, int chunk,
+                                        int KB, int NB, Tile &next, int &next_step, int &t_next, int &ahead,
                                         const uint8_t *&a, const uint8_t *&b,
                                         uint32_t (&src)[S::kLoads], uint32_t &scale_src) {
   ++ahead;
-  a += kScaleBlock;
-  b += kScaleBlock;
-  if (++next_kb < KB) return;
-  next_kb = 0;
+  a += KS * kScaleBlock;
+  b += KS * kScaleBlock;
+  if (++next_step * KS < KB) return;
+  next_step = 0;
   t_next += slots;
   if (t_next < end) {
     next = map.find(t_next);
-    a = p.a;
-    b = p.b + static_cast<size_t>(next.e) * p.N * p.K;
+    a = p.a + ks * kScaleBlock;
+    b = p.b + static_cast<size_t>(next.e) * p.N * p.K + ks * kScaleBlock;
     tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
   } else {
     next.e = -1;
@@ -273,13 +276,13 @@ __device__ __forceinline__ void advance(const Gemm8Args &p, const TileMap<BM> &m
 
 // Persistent: a workgroup per CU (or two, of small tiles) runs tiles one behind the other, and the steps of all of them are
 // one stream: the next tile's first loads are on their way while this one's last products and its epilogue run.
-template <int BM, int BN, int WM, int WN, int NS, int kOut>
-__global__ void __launch_bounds__(WM * WN * 64, 2)
+template <int BM, int BN, int WM, int WN, int NS, int KS, int kOut>
+__global__ void __launch_bounds__(KS * WM * WN * 64, 2)
 gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
-  using S = TileShape<BM, BN, WM, WN, NS>;
+  using S = TileShape<BM, BN, WM, WN, NS, KS>;
   using Out = std::conditional_t<kOut == kGemm8Bf16, bf16_t, half_t>;
-  extern __shared__ __attribute__((aligned(1024))) char s_tile[];          // the places, then the tile map
-  int *s_map = reinterpret_cast<int *>(s_tile + NS * S::kStage);
+  extern __shared__ __attribute__((aligned(1024))) char s_tile[];          // the places, where the groups meet, the tile map
+  int *s_map = reinterpret_cast<int *>(s_tile + S::kMap);
   TileMap<BM>::build(p, part, s_map, s_map + p.E + 1);
   __syncthreads();
   const TileMap<BM> map{s_map, s_map + p.E + 1, p.E, n_tiles};
@@ -289,7 +292,8 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
   int t_next = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (t_next >= end) return;
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ks = KS > 1 ? wave_all / S::kWaves : 0, wave = KS > 1 ? wave_all % S::kWaves : wave_all;
   const int r16 = lane & 15, g = lane >> 4;
   const int wm = wave / WN, wn = wave % WN;
   const int KB = scale_blocks(p.K), NB = scale_blocks(p.N), tail = p.K % kScaleBlock;
@@ -300,40 +304,44 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
   const bool scales_of_rows = wave < BM / 64, scales_of_columns = wave == BM / 64;       // lane i: of column 128 i
   const float *scale_base = p.b_scale;
   if (scales_of_rows) scale_base = p.a_scale;
-  // the step whose loads are issued next: tile `next` (e < 0: there is none), block next_kb
-  int t_now = t_next, next_kb = 0, ahead = 0;        // ahead: steps loaded beyond the one that is computed
+  // the step whose loads are issued next: tile `next` (e < 0: there is none), block KS next_step + ks
+  int t_now = t_next, next_step = 0, ahead = 0;        // ahead: steps loaded beyond the one that is computed
   Tile next = map.find(t_next);
-  const uint8_t *a = p.a, *b = p.b + static_cast<size_t>(next.e) * p.N * p.K;
+  const uint8_t *a = p.a + ks * kScaleBlock, *b = p.b + static_cast<size_t>(next.e) * p.N * p.K + ks * kScaleBlock;
   tile_sources<S, BM, BN>(p, next, wave, lane, chunk, KB, NB, src, scale_src);
-  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)s_tile));
+  char *s_mine = s_tile + ks * S::kStage;
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)s_mine));
   // Its loads in four parts: a wavefront that issues all at once waits for the queue, and its products with it.  A wavefront
   // of few products, which are done before its instructions are issued, has fewer of those with all loads in one.
   constexpr int kParts = S::TT >= 4 ? 4 : 1;
   constexpr std::integral_constant<int, 0> kFirst{};
   auto load_part = [&](int place, auto PART) __attribute__((always_inline)) {
     constexpr int quarter = decltype(PART)::value;
-    const uint32_t at = __builtin_amdgcn_readfirstlane(lds + place * S::kStage + wave * 1024);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds + place * S::kPlace + wave * 1024);
+    // (a group that has no block left loads the last one, for nothing)
+    const int kb = KS * next_step + ks, over = KS > 1 && kb >= KB ? kb - KB + 1 : 0;
+    const uint8_t *rows = a - over * kScaleBlock, *columns = b - over * kScaleBlock;
     constexpr int lo = quarter * S::kLoads / kParts, hi = (quarter + 1) * S::kLoads / kParts;
-    if (tail && next_kb == KB - 1) {
+    if (tail && kb - over == KB - 1) {
       // chunks behind the end of K: zeros for the rows, and for the columns the block's first chunk again (what is no
       // number there is no number in the sum anyway)
       const bool behind = chunk * 16 >= tail;
 #pragma unroll
       for (int i = lo; i < hi; ++i) {
-        const uint8_t *q = a + (static_cast<uint64_t>(src[i]) << 4);
+        const uint8_t *q = rows + (static_cast<uint64_t>(src[i]) << 4);
         if (i < S::kLoadsX) load16_to_lds(behind ? reinterpret_cast<const uint8_t *>(&kZeros16) : q, at + i * S::kWaves * 1024);
-        else load16_to_lds(b, src[i] - (behind ? chunk * 16 : 0), at + i * S::kWaves * 1024);
+        else load16_to_lds(columns, src[i] - (behind ? chunk * 16 : 0), at + i * S::kWaves * 1024);
       }
     } else {
 #pragma unroll
       for (int i = lo; i < hi; ++i) {
-        if (i < S::kLoadsX) load16_to_lds(a + (static_cast<uint64_t>(src[i]) << 4), at + i * S::kWaves * 1024);
-        else load16_to_lds(b, src[i], at + i * S::kWaves * 1024);
+        if (i < S::kLoadsX) load16_to_lds(rows + (static_cast<uint64_t>(src[i]) << 4), at + i * S::kWaves * 1024);
+        else load16_to_lds(columns, src[i], at + i * S::kWaves * 1024);
       }
     }
     if (quarter == 0 && (scales_of_rows || scales_of_columns))          // the wavefronts' 64 scales each, one behind the other
-      load4_to_lds(scale_base + next_kb + scale_src,
-                   __builtin_amdgcn_readfirstlane(lds + place * S::kStage + S::kRowsBytes + wave * 256));
+      load4_to_lds(scale_base + (kb - over) + scale_src,
+                   __builtin_amdgcn_readfirstlane(lds + place * S::kPlace + S::kRowsBytes + wave * 256));
   };
 
   const int x_at = (wm * (BM / WM) + r16) * kScaleBlock + (g ^ (r16 & 7)) * 16;
@@ -399,10 +407,10 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
   for (int i = 0; i < NS - 1; ++i)
     if (next.e >= 0) {
       in_turn(std::make_integer_sequence<int, kParts>{}, [&](auto I) __attribute__((always_inline)) { load_part(i, I); });
-      advance<S, BM, BN>(p, map, end, slots, wave, lane, chunk, KB, NB, next, next_kb, t_next, ahead, a, b, src, scale_src);
+      advance<S, BM, BN, KS>(p, map, end, slots, ks, wave, lane, chunk, KB, NB, next, next_step, t_next, ahead, a, b, src, scale_src);
     }
   auto on = [&]() __attribute__((always_inline)) {
-    advance<S, BM, BN>(p, map, end, slots, wave, lane, chunk, KB, NB, next, next_kb, t_next, ahead, a, b, src, scale_src);
+    advance<S, BM, BN, KS>(p, map, end, slots, ks, wave, lane, chunk, KB, NB, next, next_step, t_next, ahead, a, b, src, scale_src);
   };
   auto begin_load = [&](int place) __attribute__((always_inline)) {
     --ahead;                                         // (which counted the step that comes)
@@ -412,21 +420,21 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
   };
   meet();
   begin_load(NS - 1);
-  sb = *reinterpret_cast<const float *>(s_tile + sb_at);
+  sb = *reinterpret_cast<const float *>(s_mine + sb_at);
 #pragma unroll
   for (int t = 0; t < S::TT; ++t) {
-    x[t] = fragment(s_tile, x_at, t);
-    sa[t] = *reinterpret_cast<const float *>(s_tile + sa_at + 64 * t);
+    x[t] = fragment(s_mine, x_at, t);
+    sa[t] = *reinterpret_cast<const float *>(s_mine + sa_at + 64 * t);
   }
 #pragma unroll
-  for (int c = 0; c < kRing - 1; ++c) w[c] = fragment(s_tile, w_at, c);
+  for (int c = 0; c < kRing - 1; ++c) w[c] = fragment(s_mine, w_at, c);
   clear();
 
-  int place = 0, kb = 0;
+  int place = 0, step = 0;
   while (true) {
-    const char *now = s_tile + place * S::kStage;
+    const char *now = s_mine + place * S::kPlace;
     const int coming = place + 1 < NS ? place + 1 : 0;
-    const char *next_place = s_tile + coming * S::kStage;            // behind the last step: read for nothing
+    const char *next_place = s_mine + coming * S::kPlace;            // behind the last step: read for nothing
     in_turn(std::make_integer_sequence<int, S::CT>{}, [&](auto C) __attribute__((always_inline)) {
       constexpr int c = decltype(C)::value, c_ahead = c + kRing - 1;
       constexpr bool at_meet = c == S::CT - kRing + 1, rows_here = S::TT >= 4 && c == S::CT - 1;
@@ -448,7 +456,7 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
         const int q = c * S::TT + t;
         if (q == kLate) {
 #pragma unroll
-          for (int i = 0; i < S::TT; ++i) s[i] = sa[i] * sb;
+          for (int i = 0; i < S::TT; ++i) s[i] = KS == 1 || KS * step + ks < KB ? sa[i] * sb : 0.0f;
         }
         product[q % (kLate + 1)] = mfma8(w[c % kRing], x[t]);
         scaled((q + Q - kLate) % Q);
@@ -482,12 +490,30 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
       for (int t = 0; t < S::TT; ++t) x[t] = x_next[t];
     }
     place = coming;
-    if (++kb < KB) continue;
+    if (++step * KS < KB) continue;
 
     // the tile's end.  A lane holds one row and, in every product, four consecutive columns; of four products' columns it
     // stores 16 consecutive ones, which it gets from the lanes that hold the same row
 #pragma unroll
     for (int q = Q - kLate; q < Q; ++q) scaled(q);
+    if constexpr (KS > 1) {
+      static_assert(KS == 2, "two groups meet");
+      // (written again only behind barriers of the next tile's steps)
+      float4v *at = reinterpret_cast<float4v *>(s_tile + NS * S::kPlace) + wave * Q * 64 + lane;
+      if (ks == 1) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) at[q * 64] = acc[q / S::TT][q % S::TT];
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);            // lgkmcnt(0)
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (ks == 0) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) acc[q / S::TT][q % S::TT] += at[q * 64];
+      }
+    }
+    if (KS == 1 || ks == 0) {
     const int rows = tile.rows < BM ? tile.rows : BM, n0 = tile.n * BN;
     const Out *bias = p.bias ? static_cast<const Out *>(p.bias) + static_cast<size_t>(tile.e) * p.N : nullptr;
     const int col0 = n0 + wn * (BN / WN), nb = block_of(col0);       // a wavefront's columns share a scale
@@ -556,10 +582,11 @@ gemm8_tile_kernel(Gemm8Args p, int n_tiles, int part) {
         }
       }
     }
+    }
     t_now += slots;
     if (t_now >= end) return;
     tile = map.find(t_now);
-    kb = 0;
+    step = 0;
     clear();
   }
 }
@@ -791,11 +818,11 @@ int compute_units() {
   return cached;
 }
 
-template <int BM, int BN, int WM, int WN, int NS, int kOut>
+template <int BM, int BN, int WM, int WN, int NS, int KS, int kOut>
 int launch_tiles(const Gemm8Args &p, int part, hipStream_t st, const char *what) {
-  using S = TileShape<BM, BN, WM, WN, NS>;
-  auto kernel = gemm8_tile_kernel<BM, BN, WM, WN, NS, kOut>;
-  const size_t lds = NS * S::kStage + 4 * (3 * p.E + 1);
+  using S = TileShape<BM, BN, WM, WN, NS, KS>;
+  auto kernel = gemm8_tile_kernel<BM, BN, WM, WN, NS, KS, kOut>;
+  const size_t lds = S::kMap + 4 * (3 * p.E + 1);
   const int cus = compute_units(), n_tiles = (p.N + BN - 1) / BN;
   CCF_REQUIRE(cus > 0, CCF_ERR_HIP, "%s: no device", what);
   if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), lds, what)) return rc;
@@ -819,25 +846,29 @@ int launch_split(const Gemm8Args &p, hipStream_t st, const char *what) {
 
 // The form by sizes; the experts' row counts are on the device, so their loads are taken as even, and a quarter more.  The
 // limits are where measured times cross (us, K -> N, rows of an expert; weights cycled through a graph's replays):
-//   K over wavefronts, for at most 32 rows, where one round of workgroups holds them and K is long: 4096 -> 14336, 1 row
-//   14.8 and tiles of 64 21.7; 8192 -> 2048 of 8 experts, 8 rows 26 and 40; but 768 -> 2048 7.8 and 6.9, and in two rounds
-//   (14336 -> 4096 of 8, 2 rows) 86 and 77.
-//   Tiles of 64, while there are few tiles: 4096 -> 1024, 512 rows 22, of 128 28, of 256 51; 4096 -> 14336, 333 rows 47, 41, 56.
+//   K over wavefronts, for at most 16 rows, where one round of workgroups holds them and K is long: 4096 -> 14336, 1 row
+//   14.7 and tiles of 64 in two groups 18.4; 8192 -> 2048 of 8 experts, 8 rows 26 and 31; but 4096 -> 1024, 32 rows 19.5 and
+//   16.6, 768 -> 2048 7.8 and 6.7, and in two rounds (14336 -> 4096 of 8, 2 rows) 86 and, tiles of 64, 77.
+//   Tiles of 64, while there are few tiles: 4096 -> 1024, 512 rows 22, of 128 28, of 256 51; 4096 -> 14336, 333 rows 47, 41, 56;
+//   in two groups while a CU has one at most: 17 for 22, 4096 -> 1024 of 8 experts, 139 rows 20 for 23; with a tile on each of
+//   256 CUs that wait for weights (14336 -> 4096 of 8) 96 for 77.
 //   Tiles of 256 with the rest as a launch of its own, where the whole tiles alone fill the chip: 4096 -> 14336 of 8, 512
 //   rows 364, all in tiles of 256 394, of 128 397; but 4096 -> 1024, 4096 rows 56, 54, 32.
 //   Tiles of 256, where tiles of 128 go over a round: 4096 -> 14336, 700 rows 60, of 128 68; 512 rows 56 and 45.
-enum Form { kSplit = 1, kTiles256, kTiles128, kTiles64, kTilesAndRest };
+enum Form { kSplit = 1, kTiles256, kTiles128, kTiles64, kTilesAndRest, kTiles64Halves };
+constexpr long long kOneEach = 192;                  // of 256 CUs have a tile: few enough that two groups to a CU pay
 Form form_of(const Gemm8Args &p) {
   constexpr long long kCus = 256;
   const bool grouped = p.offsets != nullptr;
   const long long owners = grouped ? (p.E < p.max_rows ? p.E : p.max_rows) : 1;
   const long long rows = (p.max_rows + owners - 1) / owners, likely = grouped ? rows + rows / 4 : rows;
   auto tiles = [&](int bm, int bn) { return owners * ((likely + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-  if (p.K >= 2048 && (grouped ? 2 * rows : rows) <= 32 && owners * ((p.N + 63) / 64) <= kCus) return kSplit;
+  if (p.K >= 2048 && (grouped ? 2 * rows : rows) <= 16 && owners * ((p.N + 63) / 64) <= kCus) return kSplit;
   if (owners * (rows / kWholeRows) * ((p.N + 255) / 256) >= kCus) {
     const long long rest = rows % kWholeRows;
     return grouped || (rest > 0 && rest <= kLeftRows) ? kTilesAndRest : kTiles256;          // an empty launch is 4 us
   }
+  if (tiles(64, 128) <= kOneEach) return kTiles64Halves;
   if (likely <= 64 || tiles(64, 128) <= 448) return kTiles64;
   if (likely > 128 && tiles(128, 128) >= 640) return kTiles256;
   return kTiles128;
@@ -848,18 +879,18 @@ int gemm8_out(const Gemm8Args &p, hipStream_t st, const char *what) {
   // (the 8-bit output wants all 128 columns of a scale in one workgroup)
   constexpr int CS = kOut == kGemm8Gelu8 ? 2 : 1;
   switch (g_fp8_form ? static_cast<Form>(g_fp8_form) : form_of(p)) {
-    case kSplit: {
-      // 16 rows at a time, or 32 where an expert probably has more
-      const int rows = p.offsets ? 2 * ((p.max_rows + p.E - 1) / p.E) : p.max_rows;
-      return rows <= 16 ? launch_split<1, 4, CS, kOut>(p, st, what) : launch_split<2, 4, CS, kOut>(p, st, what);
-    }
-    case kTiles256: return launch_tiles<256, 256, 4, 2, 2, kOut>(p, kAll, st, what);
-    case kTiles128: return launch_tiles<128, 128, 4, 1, 2, kOut>(p, kAll, st, what);
-    case kTiles64: return launch_tiles<64, 128, 4, 1, 3, kOut>(p, kAll, st, what);
-    default: break;
+    case kSplit: return launch_split<1, 4, CS, kOut>(p, st, what);
+    case kTiles256: return launch_tiles<256, 256, 4, 2, 2, 1, kOut>(p, kAll, st, what);
+    case kTiles128: return launch_tiles<128, 128, 4, 1, 2, 1, kOut>(p, kAll, st, what);
+    case kTiles64: return launch_tiles<64, 128, 4, 1, 3, 1, kOut>(p, kAll, st, what);
+    case kTiles64Halves: return launch_tiles<64, 128, 4, 1, 2, 2, kOut>(p, kAll, st, what);
+    case kTilesAndRest: break;
   }
-  if (int rc = launch_tiles<256, 256, 4, 2, 2, kOut>(p, kWhole, st, what)) return rc;
-  return launch_tiles<64, 128, 4, 1, 3, kOut>(p, kLeft, st, what);
+  if (int rc = launch_tiles<256, 256, 4, 2, 2, 1, kOut>(p, kWhole, st, what)) return rc;
+  // (one expert in four has so few rows left, loads being arbitrary)
+  const long long left = (p.offsets ? (p.E + 3) / 4 : 1) * static_cast<long long>((p.N + 127) / 128);
+  return left <= kOneEach ? launch_tiles<64, 128, 4, 1, 2, 2, kOut>(p, kLeft, st, what)
+                          : launch_tiles<64, 128, 4, 1, 3, 1, kOut>(p, kLeft, st, what);
 }
 
 }  // namespace

@@ -99,7 +99,8 @@ const char *ccf_last_error(void);
  *                     of two), and the routing stage is then one launch.  0 = always histogram, scan, pos
  *   "fp8_form"        products in 8 bits: 0 (default) = form chosen by sizes; 1 = K cut over the wavefronts of a
  *                     workgroup; 2, 3, 4 = tiles of 256, 128, 64 rows through LDS; 5 = tiles of 256, and an
- *                     expert's last 64 rows or fewer beyond them in a launch of their own
+ *                     expert's last 64 rows or fewer beyond them in a launch of their own; 6 = tiles of 64 rows
+ *                     by two groups of wavefronts that halve K
  *   "gate_slots"      0, 1, 2 or 4: parts of K a gate wavefront works on at a time, which divides the tokens
  *                     of a workgroup by the same number (0 = chosen by the token count)
  *   "dgrad_transpose" 0/1: the backward's input-gradient GEMM runs on a transposed copy of the

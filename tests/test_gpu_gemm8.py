@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
-@pytest.fixture(params=[0, 1, 2, 3, 4, 5], ids=["by_rule", "k_over_wavefronts", "tiles", "tiles_of_128", "tiles_of_64", "tiles_and_rest"],
+@pytest.fixture(params=range(7), ids=["by_rule", "k_over_wavefronts", "tiles", "tiles_of_128", "tiles_of_64", "tiles_and_rest", "two_groups"],
                 autouse=True)
 def form(request):
     """Every test in the form that the library picks, and in each of them."""
