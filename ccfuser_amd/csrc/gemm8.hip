@@ -102,19 +102,19 @@ __device__ __forceinline__ Tile find_tile(const Gemm8Args &p, int pid, int grid,
 
 // ------------------------------------------------------------------ tiles through LDS
 //
-// BM rows x BN columns, WM x WN wavefronts; a K step is a block of 128, staged by direct loads into one of two LDS places
-// while the other is multiplied (of the small tile three, so that a load has two steps to land).  16-byte chunks of a row lie at chunk ^ (row % 8), which the loads' global addresses apply,
-// and a lane's two chunks are g and g + 4 (g = lane / 16): a read then takes 5 cycles of a wavefront (256 bytes each),
-// with 2 g and 2 g + 1 9, unswizzled 17.  The scales of a step come the same way, a
-// lane per row, and lie by row.
+// BM rows x BN columns, WM x WN wavefronts; a K step is a block of 128, staged by direct loads into one of NS LDS places
+// while another is multiplied (two; of the 64-row tile in one group three, so that a load has two steps to land).  16-byte
+// chunks of a row lie at chunk ^ (row % 8), which the loads' global addresses apply, and a lane's two chunks are g and g + 4
+// (g = lane / 16): a read then takes 5 cycles of a wavefront (256 bytes each), with 2 g and 2 g + 1 9, unswizzled 17.  The
+// scales of a step come the same way, a lane per row, and lie by row.
 //
-// A wavefront reads its rows' fragments once a step and its columns' one by one, two in turn.  The step's one barrier stands
-// in front of its last columns, whose fragment is in registers by then: behind it this step's place is free for the loads
-// of the step after the next, and the next step's rows are read between the last products, each into the registers that a
-// product has just let go.  So the matrix cores run through the steps, and a load has a whole step to land.
+// A wavefront reads its rows' fragments once a step and its columns' one by one, each ahead of its products.  The step's one
+// barrier stands in front of its last columns, whose fragments are in registers by then: behind it this step's place is free
+// for the loads of the step NS on, and the next step's rows are read between the last products.  So the matrix cores run
+// through the steps, and a load has a whole step to land.
 //
 // KS = 2: two groups of such wavefronts take every other block each, with places of their own, and their sums meet in LDS at
-// the tile's end: half as many steps, for a CU that has one small tile.
+// the tile's end: half as many steps, for a CU that has one small tile (512 rows, 4096 -> 1024: 17 us for 21.5).
 template <int BM, int BN, int WM, int WN, int NS, int KS>
 struct TileShape {
   static constexpr int kWaves = WM * WN, kThreads = KS * kWaves * 64;       // (wavefronts of a group)
